@@ -438,6 +438,55 @@ NSA_API size_t nsa_incremental_workspace_bytes(const nsa_decode_desc* desc);
 NSA_API size_t nsa_incremental_workspace_min_bytes(const nsa_decode_desc* desc);      /* as for the layer's forward */
 NSA_API int nsa_incremental_fwd(const nsa_decode_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Paged serving: requests of any lengths in one step, their keys and values held in 4 bits (the reference has no counterpart).
+ *
+ * A page holds 64 tokens of all G kv groups; cache is [n_pages][G][nsa_cache4_page_bytes] bytes, 16-byte aligned.  A page of one
+ * group is four records of 16 tokens; a record holds 256 bytes of codes per 32 dimensions (those of the keys first, then those of
+ * the values), then 16 fp16 scales for each.  Keys: byte 8 (4 n + j) + 4 t holds the first of four bytes with dimensions 8 j + e (e the nibble,
+ * low ones first) of token 8 t + n.  Values: byte 8 (4 n + j) + 2 (2 t + b) the first of two with dimensions 8 e + n of token 8 t + 2 j + b.
+ * Scales: place 4 j + 2 t + b belongs to token 8 t + 2 j + b.  A code c stands for (c - 8) s; s is a seventh of the largest magnitude of its
+ * 32 values, rounded to 8 significant bits (multiples of 2^-24 at the low end), c - 8 the value over s rounded to nearest even, within -7..7.
+ * Magnitudes above 57120 (infinities) are held as that, NaN as 0.  dk and dv are multiples of 32 up to 256 (page_bytes is 0 else).
+ * Slot s is token s % 64 of page s / 64.
+ *
+ * nsa_block_tables lays out a step: request r has cached[r] tokens in the cache and brings fresh[r] more.  Its row of table [S, P] (rows
+ * table_ld apart) holds the pages of what is cached; pages that the new tokens open come from the front of free_pages [F], in the order
+ * of the requests, and are written into the table.  slots and positions [N] list the new tokens one request after the other (-1 behind
+ * the last, N is at least their number), starts [S + 1] where each request's begin, lengths [S] the tokens it then has, pages [1] how
+ * many pages the step takes.  Where that is more than F, or a table row is too short, tokens without a page have slot -1 (and
+ * table entries -1): the caller compares pages with F.  Negative lengths count as 0.  At most 16384 requests a call.
+ *
+ * nsa_cache4_append: k [N,G,dk] and v [N,G,dv] (strides6: token, group, dimension of each) into their slots; slots outside the cache are
+ * passed over.  Slots of one call are distinct (a slot given twice holds bytes of both tokens).  nsa_cache4_read: the values that the
+ * slots hold, k [N,G,dk] and v [N,G,dv] contiguous and 16-byte aligned; zeros for slots outside the cache.
+ *
+ * nsa_cache4_attn_fwd: q [N,H,dk] (strides sq: token, head; unit stride within a head), tokens starts[r] .. starts[r+1]-1 being the
+ * newest ones of request r with lengths[r] tokens.  The token at position p sees keys j <= p; with window > 0 also j > p - window; with
+ * n_sel > 0 those in the 64-key blocks indices[token][group][0..n_sel) (int32, contiguous; negative ones and repetitions do not count),
+ * n_sel <= 32.  Pages that the table does not give (entries outside 0..n_pages-1, positions behind its P pages) are not seen.  out [N,H,dv]
+ * contiguous in the type of q; L, M [N,H] as above; rows that see nothing are 0, L = M = -inf.  Rows behind the last request's are left as
+ * they were.  max_new: no request has more new tokens than this (0: not known); it only chooses between kernels. */
+NSA_API int nsa_block_tables(const int32_t* cached, const int32_t* fresh, int32_t* table, int64_t table_ld, const int32_t* free_pages,
+                             int64_t* slots, int32_t* positions, int32_t* starts, int32_t* lengths, int32_t* pages, int S, int P, int F,
+                             int N, int page_tokens, void* stream);
+NSA_API size_t nsa_cache4_page_bytes(int dk, int dv);
+NSA_API int nsa_cache4_append(const void* k, const void* v, const int64_t* strides6, const int64_t* slots, void* cache, int N, int n_pages,
+                              int G, int dk, int dv, int dtype, void* stream);
+NSA_API int nsa_cache4_read(const void* cache, const int64_t* slots, void* k, void* v, int N, int n_pages, int G, int dk, int dv, int dtype,
+                            void* stream);
+typedef struct nsa_cache4_desc {
+  int N, S, P, H, G, dk, dv, n_pages, n_sel, window, max_new, dtype;
+  float scale;
+  int64_t sq[2], table_ld;
+  const void *q, *cache;
+  const int32_t *table, *lengths, *starts, *indices;
+  void* out;
+  float *L, *M;
+} nsa_cache4_desc;
+NSA_API size_t nsa_cache4_attn_workspace_bytes(const nsa_cache4_desc* desc);
+NSA_API int nsa_cache4_attn_fwd(const nsa_cache4_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

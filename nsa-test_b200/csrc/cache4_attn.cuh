@@ -1,0 +1,218 @@
+// Attention over the 4-bit paged cache: how the work is cut up, shared by its kernels.
+//
+// A segment is what one softmax runs over for one tile of rows: (request, kv group, tile of ROWS rows), a row being one query token and
+// one of the group's heads; in the selected form (token, kv group, tile).  Its units are pages of 64 keys (selected form: places of the
+// token's block list).  The units of all segments, one after the other, are dealt to the thread blocks in equal shares, wherever the
+// segments end: requests of any mixture of lengths keep every SM busy to the end.  A block merges what it has of a segment; a segment
+// that one block has whole goes straight to the output, the others leave partial results (running maximum, sum and unnormalised
+// output, 32 bits) that combine_kernel joins in order.  A block has at most two partial segments, its first and its last.  Nothing is
+// known of the lengths on the host: every block forms the prefix sums over the requests for itself.
+#pragma once
+#include "cache4.cuh"
+
+namespace nsa {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kSelMax = 32;          // places of a block list: one per lane
+
+struct Segment {
+  int tok0;        // first token of the request among the step's (selected form: the token)
+  int row0, nrows; // first flattened row (token * heads per group + head) within the request and how many there are
+  int r, g;
+  int pos0;        // position of token tok0
+  int lo, hi;      // units
+};
+
+// what a block leaves about its last segment, if the segment starts there and ends in a later block
+struct SplitRecord {
+  int open, tok0, row0, nrows, g, pad;
+  long long first, last, total;      // the segment's units and the number of all
+};
+
+__device__ __forceinline__ long long share(long long total, int c, int n) { return total * c / n; }
+
+template <int ROWS>
+struct Walk {
+  const Cache4Args& a;
+  Segment s;
+  int tile, tiles, len, fresh;       // of the current request
+  long long total;
+
+  __device__ Walk(const Cache4Args& args) : a(args) {}
+
+  __device__ __forceinline__ int row_tiles(int n) const { return (n * a.hpg + ROWS - 1) / ROWS; }
+  // tokens and length of a request: nothing outside [0, N] whatever the arrays hold
+  __device__ __forceinline__ void request(int r, int& tok0, int& n, int& length) const {
+    const int b = min(max(a.starts[r], 0), a.N), e = min(max(a.starts[r + 1], 0), a.N);
+    tok0 = b;
+    n = max(e - b, 0);
+    if (n * a.hpg < a.rows_lo || n * a.hpg >= a.rows_hi) n = 0;
+    length = min(max(a.lengths[r], 0), 1 << 30);
+  }
+  // pages that some row of tile t can see (at least one, so that every row is written)
+  __device__ __forceinline__ void pages(int length, int n, int t, int& lo, int& hi) const {
+    const int p0 = length - n;
+    const int first = p0 + t * ROWS / a.hpg, last = p0 + min(n * a.hpg - 1, t * ROWS + ROWS - 1) / a.hpg;
+    hi = last < 0 ? 0 : min(last / kPageTokens + 1, a.P);
+    lo = a.window > 0 ? max(first - a.window + 1, 0) / kPageTokens : 0;
+    if (hi <= lo) { lo = 0; hi = 1; }
+  }
+  __device__ __forceinline__ long long units(int r) const {
+    int tok0, n, length;
+    long long sum = 0;
+    request(r, tok0, n, length);
+    for (int t = 0, m = row_tiles(n); t < m; ++t) {
+      int lo, hi;
+      pages(length, n, t, lo, hi);
+      sum += hi - lo;
+    }
+    return sum * a.G;
+  }
+
+  __device__ __forceinline__ void set_tile() {
+    s.row0 = tile * ROWS;
+    if (a.n_sel) {
+      s.nrows = min(ROWS, a.hpg - s.row0);
+      return;
+    }
+    s.nrows = min(ROWS, fresh * a.hpg - s.row0);
+    pages(len, fresh, tile, s.lo, s.hi);
+  }
+  __device__ __forceinline__ void set_request(int r) {
+    s.r = r;
+    request(r, s.tok0, fresh, len);
+    s.pos0 = len - fresh;
+    tiles = row_tiles(fresh);
+  }
+  // selected form: request and position of token s.tok0, given that it belongs to s.r or a later one
+  __device__ __forceinline__ void set_token() {
+    while (s.r + 1 < a.S && a.starts[s.r + 1] <= s.tok0) ++s.r;
+    s.pos0 = a.lengths[s.r] - a.starts[s.r + 1] + s.tok0;
+  }
+
+  // Number of all units; all threads of the block take part.  Blocks of T threads, scratch of T / 32 + 3 long longs in shared memory.
+  template <int T>
+  __device__ __forceinline__ void start(long long* scratch) {
+    if (a.n_sel) {
+      const int n = min(max(a.starts[a.S], 0), a.N);
+      tiles = (a.hpg + ROWS - 1) / ROWS;
+      total = (long long)n * a.G * tiles * a.n_sel;
+      s.lo = 0;
+      s.hi = a.n_sel;
+      return;
+    }
+    long long x = 0;
+    for (int r = threadIdx.x; r < a.S; r += T) x += units(r);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < T / 32; ++w) total += scratch[w];
+    __syncthreads();
+  }
+  // Segment that unit u (< total) lies in; returns its place within the segment.
+  template <int T>
+  __device__ __forceinline__ int seek(long long u, long long* scratch) {
+    if (a.n_sel) {
+      const long long seg = u / a.n_sel;
+      tile = (int)(seg % tiles);
+      s.g = (int)(seg / tiles % a.G);
+      s.tok0 = (int)(seg / tiles / a.G);
+      int lo = 0, up = a.S;                     // last request that starts at or before the token: 32 probes at a time
+      while (up - lo > 1) {
+        const int step = (up - lo + 31) / 32, at = lo + (threadIdx.x & 31) * step;
+        const unsigned le = __ballot_sync(0xffffffffu, at < up && a.starts[at < up ? at : lo] <= s.tok0);
+        const int k = max(31 - __clz(le), 0);
+        up = min(up, lo + (k + 1) * step);
+        lo += k * step;
+      }
+      s.r = lo;
+      set_token();
+      set_tile();
+      return (int)(u % a.n_sel);
+    }
+    long long run = 0;
+    for (int base = 0; base < a.S; base += T) {
+      const int r = base + threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+      const long long x = r < a.S ? units(r) : 0;
+      long long p = x;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, p, o);
+        if (lane >= o) p += y;
+      }
+      __syncthreads();
+      if (lane == 31) scratch[warp] = p;
+      if (threadIdx.x == 0) scratch[T / 32] = -1;
+      __syncthreads();
+      long long before = run;
+      for (int w = 0; w < T / 32; ++w) {
+        if (w < warp) before += scratch[w];
+        run += scratch[w];
+      }
+      p += before;
+      if (u >= p - x && u < p) {
+        scratch[T / 32] = r;
+        scratch[T / 32 + 1] = u - (p - x);
+      }
+      __syncthreads();
+      if (scratch[T / 32] >= 0) break;
+    }
+    set_request((int)scratch[T / 32]);
+    long long off = scratch[T / 32 + 1];
+    __syncthreads();
+    const long long per = units(s.r) / a.G;
+    s.g = (int)(off / per);
+    int place = (int)(off % per);
+    for (tile = 0;; ++tile) {
+      set_tile();
+      if (place < s.hi - s.lo || tile + 1 >= tiles) return place;
+      place -= s.hi - s.lo;
+    }
+  }
+  // the segment after this one (there is one)
+  __device__ __forceinline__ void next() {
+    if (++tile < tiles) return set_tile();
+    tile = 0;
+    if (++s.g < a.G) return set_tile();
+    s.g = 0;
+    if (a.n_sel) {
+      ++s.tok0;
+      set_token();
+      return set_tile();
+    }
+    for (int r0 = s.r + 1; r0 < a.S; r0 += 32) {          // 32 requests at a time: other launches may own long runs of them
+      const int r = r0 + (threadIdx.x & 31);
+      int tok0, n = 0, length;
+      if (r < a.S) request(r, tok0, n, length);
+      const unsigned some = __ballot_sync(0xffffffffu, n > 0);
+      if (some) {
+        set_request(r0 + __ffs(some) - 1);
+        return set_tile();
+      }
+    }
+  }
+};
+
+// Workspace: records of all blocks, then two partial results a block: [rows][dv] unnormalised outputs, [rows] (maximum, sum).
+__host__ __device__ __forceinline__ size_t split_rec_bytes(int blocks) { return ((size_t)blocks * sizeof(SplitRecord) + 255) / 256 * 256; }
+__host__ __device__ __forceinline__ size_t split_part_floats(int rows, int dv) { return (size_t)rows * (dv + 2); }
+__host__ __device__ __forceinline__ size_t split_bytes(int blocks, int rows, int dv) {
+  return split_rec_bytes(blocks) + (size_t)blocks * 2 * split_part_floats(rows, dv) * 4;
+}
+__device__ __forceinline__ float* split_part(const Cache4Args& a, int blocks, int rows, int block, int which) {
+  return reinterpret_cast<float*>(a.ws + split_rec_bytes(blocks)) + ((size_t)block * 2 + which) * split_part_floats(rows, a.dv);
+}
+
+// row i of a segment: its token and head
+__device__ __forceinline__ int64_t out_row(const Cache4Args& a, const Segment& s, int i) {
+  const int f = s.row0 + i;
+  return (int64_t)(s.tok0 + f / a.hpg) * a.H + s.g * a.hpg + f % a.hpg;
+}
+
+int launch_combine(const Cache4Args& a, int blocks, int rows, bool f32, cudaStream_t st);
+int cache4_sm_count();
+
+}  // namespace nsa

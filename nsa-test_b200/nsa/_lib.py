@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p, POINTER
 
 import torch
@@ -46,6 +47,11 @@ class DecodeDesc(ctypes.Structure):
                 + [("sx", c_int64 * 2), ("w", c_void_p * 5), ("bias", c_void_p * 5)]
                 + [(n_, c_void_p) for n_ in ("gate_w1", "gate_b1", "gate_w2", "gate_b2", "pos_embed", "phi_w1", "phi_b1",
                                              "phi_w2", "phi_b2", "k_new")] + [("sk", c_int64 * 4)])
+
+
+# nsa_cache4_desc of include/nsa_b200.h, packed by one call (a decode step makes dozens): N, S, P, H, G, dk, dv, n_pages, n_sel, window,
+# max_new, dtype; scale; sq[2], table_ld; q, cache, table, lengths, starts, indices, out, L, M
+CACHE4_DESC = struct.Struct("=12if4x3q9Q")
 
 
 # pieces of the layer's context buffer, in the order of enum nsa_layer_ctx_piece
@@ -109,6 +115,12 @@ PROTOTYPES = {
     "nsa_gate_mix_bwd": (c_int, [_P] * 9 + [c_int] * 7 + [_P]),
     "nsa_gate_mix_bwd_delta": (c_int, [_P] * 10 + [c_int] * 7 + [_P]),
     "nsa_slc_fwd_mix": (c_int, [_P] * 7 + [_I64P] + [c_int] * 9 + [c_float, c_int, c_int, c_int] + [_P] * 5 + [c_int, c_int, _P, c_size_t, _P]),
+    "nsa_block_tables": (c_int, [_P, _P, _P, c_int64] + [_P] * 6 + [c_int] * 5 + [_P]),
+    "nsa_cache4_page_bytes": (c_size_t, [c_int, c_int]),
+    "nsa_cache4_append": (c_int, [_P, _P, _I64P, _P, _P] + [c_int] * 6 + [_P]),
+    "nsa_cache4_read": (c_int, [_P] * 4 + [c_int] * 6 + [_P]),
+    "nsa_cache4_attn_workspace_bytes": (c_size_t, [_P]),
+    "nsa_cache4_attn_fwd": (c_int, [_P, _P, c_size_t, _P]),
 }
 
 for _name, (_res, _args) in PROTOTYPES.items():

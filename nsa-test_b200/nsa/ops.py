@@ -6,6 +6,7 @@ nothing but its outputs; shapes follow the reference project's kernel-call contr
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -634,3 +635,87 @@ def layer_bwd(desc, q, kv_slc, kv_cmp, kv_win, phi, ctx, dout, shared_kv: bool):
                                 ptr(g_cmp[0]), ptr(g_cmp[1]), ptr(g_win[0]), ptr(g_win[1]), ptr(dlogits), ptr(dpos), ptr(dw1), ptr(db1),
                                 ptr(dw2), ptr(db2), ptr(ws), nbytes, stream_ptr(dev)), "nsa_layer_bwd")
     return dq, g_slc, g_cmp, g_win, dlogits, (dpos, dw1, db1, dw2, db2)
+
+
+# ------------------------------------------------------------------------------------------------
+# paged serving: block tables, the 4-bit cache, attention over it
+# ------------------------------------------------------------------------------------------------
+
+class _on:
+    """``torch.cuda.device`` that costs nothing where the device is the current one already."""
+    __slots__ = ("dev", "ctx")
+
+    def __init__(self, dev):
+        self.dev = dev
+
+    def __enter__(self):
+        self.ctx = None if torch.cuda.current_device() == self.dev.index else torch.cuda.device(self.dev)
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
+def block_tables(cached, new, table, free_pages, tokens: int, page_tokens: int):
+    """nsa_block_tables -> (slots [tokens] int64, positions [tokens], starts [S+1], lengths [S], pages [1], int32); table in place."""
+    dev = require_cuda(cached, new, table, free_pages)
+    S, P = table.shape
+    n = 2 * tokens                                    # one allocation: int64 slots first, then the int32 arrays
+    buf = torch.empty(n + tokens + 2 * S + 2, device=dev, dtype=torch.int32)
+    slots = buf[:n].view(torch.int64)
+    positions, starts, lengths, pages = buf[n:].split((tokens, S + 1, S, 1))
+    base = buf.data_ptr()
+    with _on(dev):
+        check(lib.nsa_block_tables(cached.data_ptr(), new.data_ptr(), table.data_ptr(), table.stride(0) if S > 1 else P, free_pages.data_ptr(),
+                                   base, base + 8 * tokens, base + 12 * tokens, base + 12 * tokens + 4 * (S + 1),
+                                   base + 12 * tokens + 4 * (2 * S + 1), S, P, free_pages.numel(), tokens, page_tokens, stream_ptr(dev)),
+              "nsa_block_tables")
+    return slots, positions, starts, lengths, pages
+
+
+def cache4_append(k, v, slots, cache) -> None:
+    """nsa_cache4_append: k [N,G,dk], v [N,G,dv] of any strides into the slots of cache [pages,G,page bytes]."""
+    dev = require_cuda(k, v, slots, cache)
+    N, G, dk = k.shape
+    with _on(dev):
+        check(lib.nsa_cache4_append(k.data_ptr(), v.data_ptr(), i64((*k.stride(), *v.stride())), slots.data_ptr(), cache.data_ptr(), N,
+                                    cache.shape[0], G, dk, v.shape[2], dtype_code(k), stream_ptr(dev)), "nsa_cache4_append")
+
+
+def cache4_read(cache, slots, dk: int, dv: int, dtype):
+    """nsa_cache4_read -> (k [N,G,dk], v [N,G,dv])."""
+    dev = require_cuda(cache, slots)
+    N, G = slots.numel(), cache.shape[1]
+    k = torch.empty(N, G, dk, device=dev, dtype=dtype)
+    v = torch.empty(N, G, dv, device=dev, dtype=dtype)
+    with _on(dev):
+        check(lib.nsa_cache4_read(cache.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), N, cache.shape[0], G, dk, dv, dtype_code(k),
+                                  stream_ptr(dev)), "nsa_cache4_read")
+    return k, v
+
+
+@functools.lru_cache(maxsize=4096)
+def _cache4_workspace(sizes) -> int:
+    """Scratch of an attention call over the 4-bit cache, a function of its sizes alone."""
+    return lib.nsa_cache4_attn_workspace_bytes(_lib.CACHE4_DESC.pack(*sizes, 1.0, *([0] * 12)))
+
+
+def cache4_attn(q, cache, table, lengths, starts, indices, dk: int, dv: int, window: int, scale: float, max_new: int, out=None):
+    """nsa_cache4_attn_fwd -> (out [N,H,dv], L [N,H], M [N,H]); q [N,H,dk] with unit stride within a head."""
+    dev = require_cuda(q, cache, table, lengths, starts, indices, out)
+    N, H, _ = q.shape
+    S, P = table.shape
+    if out is None:
+        out = torch.empty(N, H, dv, device=dev, dtype=q.dtype)
+    L, M = torch.empty(2, N, H, device=dev, dtype=torch.float32).unbind()
+    sizes = (N, S, P, H, cache.shape[1], dk, dv, cache.shape[0], 0 if indices is None else indices.shape[2], window, max_new, dtype_code(q))
+    nbytes = _cache4_workspace(sizes)
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    desc = _lib.CACHE4_DESC.pack(*sizes, scale, q.stride(0), q.stride(1), table.stride(0) if S > 1 else P, q.data_ptr(), cache.data_ptr(),
+                                 table.data_ptr(), lengths.data_ptr(), starts.data_ptr(), 0 if indices is None else indices.data_ptr(),
+                                 out.data_ptr(), L.data_ptr(), M.data_ptr())
+    with _on(dev):
+        check(lib.nsa_cache4_attn_fwd(desc, ws.data_ptr(), nbytes, stream_ptr(dev)), "nsa_cache4_attn_fwd")
+    return out, L, M
