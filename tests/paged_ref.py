@@ -43,13 +43,14 @@ def tables(cached, new, table, free, tokens, page):
 
 def attend(q, k, v, lengths, starts, scale, window=None, indices=None, seen_keys=None):
     """q [N,H,dk]; k, v lists of [T, G, d] per request.  -> o, L, M and the sums that bound their errors: A = sum p |v|, B = largest sum of
-    |q k| scale over the visible keys (all 64-bit; rows behind the last request: nan).  seen_keys(r): extra mask [T] of a request."""
+    |q k| scale over the visible keys, V = sum |v| over them (all 64-bit; rows behind the last request: nan).  seen_keys(r): extra mask [T]
+    of a request."""
     q = q.double()
     N, H, dk = q.shape
     G, dv = k[0].shape[1], v[0].shape[2]
     hp = H // G
     o = torch.full((N, H, dv), math.nan, dtype=torch.float64, device=q.device)
-    A, L = o.clone(), o[..., 0].clone()
+    A, V, L = o.clone(), o.clone(), o[..., 0].clone()
     M, B = L.clone(), L.clone()
     for r in range(len(lengths)):
         T = k[r].shape[0]
@@ -67,28 +68,29 @@ def attend(q, k, v, lengths, starts, scale, window=None, indices=None, seen_keys
                 hs = slice(g * hp, (g + 1) * hp)
                 kk, vv = k[r][see, g].double(), v[r][see, g].double()
                 if kk.shape[0] == 0:
-                    o[i, hs], A[i, hs], L[i, hs], M[i, hs], B[i, hs] = 0, 0, -math.inf, -math.inf, 0
+                    o[i, hs], A[i, hs], V[i, hs], L[i, hs], M[i, hs], B[i, hs] = 0, 0, 0, -math.inf, -math.inf, 0
                     continue
                 x = q[i, hs] @ kk.T * scale
                 m = x.max(1).values
                 p = torch.exp(x - m[:, None])
                 s = p.sum(1)
                 o[i, hs], A[i, hs] = p @ vv / s[:, None], p @ vv.abs() / s[:, None]
-                L[i, hs], M[i, hs] = torch.log(s), m
+                L[i, hs], M[i, hs], V[i, hs] = torch.log(s), m, vv.abs().sum(0)
                 B[i, hs] = (q[i, hs].abs() @ kk.T.abs()).max(1).values * scale
-    return o, L, M, A, B
+    return o, L, M, A, B, V
 
 
 def check(got, want, dtype, keys, dk):
     """Outputs within what the arithmetic allows.  A logit is a sum of dk products in 32 bits: off by at most dk 2^-24 B.  Relative to the
     row, probabilities are off by twice that and the sum over the keys by keys 2^-24; for bf16 queries probabilities are rounded to
-    fp16 (2^-11) and the output to bf16 (2^-8)."""
-    (o, L, M), (ro, rL, rM, A, B) = got, want
+    fp16 (by 2^-11 of themselves, below 2^-14 by 2^-25: half a step of the subnormal numbers; the row's largest is at least 1, so the sum
+    that divides them is too) and the output to bf16 (2^-8)."""
+    (o, L, M), (ro, rL, rM, A, B, V) = got, want
     rows = ~rL.isnan()
     logit = dk * 2.0 ** -24 * B + 2.0 ** -23 * rM.abs().nan_to_num(0, 0, 0)
     sums = keys * 2.0 ** -24
     rel = 2 * logit + sums + (2.0 ** -11 + 2.0 ** -20 if dtype == torch.bfloat16 else 0) + 2.0 ** -22
-    tol = rel[..., None] * A + (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -23) * ro.abs() + 1e-30
+    tol = rel[..., None] * A + (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -23) * ro.abs() + (2.0 ** -25 * V if dtype == torch.bfloat16 else 0) + 1e-30
     err = (o.double() - ro).abs()
     assert bool((err <= tol)[rows].all()), f"output off by up to {((err / tol)[rows]).max().item():.3g} of its bound"
     fin = rows & (rM > -math.inf)

@@ -403,6 +403,21 @@ def test_logits_far_apart(dtype, new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_queries_of_any_layout(dtype):
+    """Rows off 16-byte boundaries, strided dimensions, heads before tokens: through the package and straight into the library."""
+    from nsa import ops
+    H, G, dk, dv = HEADS[0]
+    s = Served([300, 70], [3, 1], H, G, dk, dv, dtype, seed=15)
+    want = ref.attend(s.q, s.k, s.v, s.lengths, s.starts, dk ** -0.5)
+    odd = torch.empty(4 * H * (dk + 1) + 1, device="cuda", dtype=dtype)[1:].view(4, H, dk + 1)[..., :dk].copy_(s.q)
+    for q in (odd, torch.empty(dk, H, 4, device="cuda", dtype=dtype).permute(2, 1, 0).copy_(s.q),
+              torch.empty(4 * H * dk + 3, device="cuda", dtype=dtype)[3:].view(4, H, dk).copy_(s.q)):
+        ref.check(s.cache.attend(q, s.table, s.len_dev, s.starts_dev), want, dtype, 300, dk)
+    ref.check(ops.cache4_attn(odd, s.cache.storage, s.table, s.len_dev, s.starts_dev, None, dk, dv, 0, dk ** -0.5, 0), want, dtype, 300, dk)
+
+
+@pytest.mark.gpu
 def test_same_bits_twice_and_on_another_stream():
     for dtype, new in ((BF, 1), (F32, 1), (BF, 50)):
         s = Served([3000, 500, 64], [new, 1, new], *HEADS[0], dtype, seed=13)
