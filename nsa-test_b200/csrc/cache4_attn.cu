@@ -462,84 +462,79 @@ __global__ void __launch_bounds__(kC4Threads, Core::kBlocksPerSm) cache4_attn_ke
   if (threadIdx.x == 0) reinterpret_cast<SplitRecord*>(a.ws)[blockIdx.x] = out;
 }
 
-// Joins the partial results of one row of one split segment: block (owner, row).  The pieces are the owner's last segment and the first
-// segments of the blocks after it; four warps take every fourth of them, in a fixed order.
+// Joins the partial results of the rows of one split segment: block (owner, first row).  The pieces are the owner's last segment and the
+// first segments of the blocks after it; four warps take every fourth of them, in a fixed order.
+constexpr int kCombineRows = 32;           // rows of an owner at once
 template <typename T>
 __global__ void __launch_bounds__(128) cache4_combine_kernel(const Cache4Args a, int blocks, int rows) {
   const SplitRecord rec = reinterpret_cast<const SplitRecord*>(a.ws)[blockIdx.x];
-  const int r = blockIdx.y;
-  if (!rec.open || r >= rec.nrows) return;
+  if (!rec.open || (int)blockIdx.y >= rec.nrows) return;
   __shared__ float acc[4][kMaxHeadDim];
   __shared__ float2 ml[4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // the last block that has a unit of the segment
-  int last = blockIdx.x;
-  {
-    int lo = blockIdx.x, up = blocks;
-    while (up - lo > 1) {
-      const int mid = (lo + up) >> 1;
-      if (share(rec.total, mid, blocks) < rec.last) lo = mid; else up = mid;
-    }
-    last = lo;
+  int last = blockIdx.x;                   // the last block that has a unit of the segment
+  for (int up = blocks; up - last > 1;) {
+    const int mid = (last + up) >> 1;
+    if (share(rec.total, mid, blocks) < rec.last) last = mid; else up = mid;
   }
-  float m = -CUDART_INF_F, l = 0.f, x[kMaxHeadDim / 32] = {};
-  for (int c = blockIdx.x + warp; c <= last; c += 4) {
-    if (c > (int)blockIdx.x && share(rec.total, c, blocks) == share(rec.total, c + 1, blocks)) continue;   // more blocks than units
-    const float* part = split_part(a, blocks, rows, c, c == (int)blockIdx.x ? 1 : 0);
-    const float2 h = reinterpret_cast<const float2*>(part + rows * a.dv)[r];
-    if (h.x == -CUDART_INF_F) continue;
-    const float mx = fmaxf(m, h.x), f0 = m == -CUDART_INF_F ? 0.f : ex2((m - mx) * kLog2e), f1 = ex2((h.x - mx) * kLog2e);
-    m = mx;
-    l = l * f0 + h.y * f1;
+  for (int r = blockIdx.y; r < rec.nrows; r += kCombineRows) {
+    float m = -CUDART_INF_F, l = 0.f, x[kMaxHeadDim / 32] = {};
+    for (int c = blockIdx.x + warp; c <= last; c += 4) {
+      if (c > (int)blockIdx.x && share(rec.total, c, blocks) == share(rec.total, c + 1, blocks)) continue;   // more blocks than units
+      const float* part = split_part(a, blocks, rows, c, c == (int)blockIdx.x ? 1 : 0);
+      const float2 h = reinterpret_cast<const float2*>(part + rows * a.dv)[r];
+      if (h.x == -CUDART_INF_F) continue;
+      const float mx = fmaxf(m, h.x), f0 = m == -CUDART_INF_F ? 0.f : ex2((m - mx) * kLog2e), f1 = ex2((h.x - mx) * kLog2e);
+      m = mx;
+      l = l * f0 + h.y * f1;
+#pragma unroll
+      for (int g = 0; g < kMaxHeadDim / 32; ++g)
+        if (g * 32 < a.dv) x[g] = x[g] * f0 + part[r * a.dv + g * 32 + lane] * f1;
+    }
+    __syncthreads();
 #pragma unroll
     for (int g = 0; g < kMaxHeadDim / 32; ++g)
-      if (g * 32 < a.dv) x[g] = x[g] * f0 + part[r * a.dv + g * 32 + lane] * f1;
-  }
+      if (g * 32 < a.dv) acc[warp][g * 32 + lane] = x[g];
+    if (lane == 0) ml[warp] = make_float2(m, l);
+    __syncthreads();
+    float M = -CUDART_INF_F, sum = 0.f, f[4];
 #pragma unroll
-  for (int g = 0; g < kMaxHeadDim / 32; ++g)
-    if (g * 32 < a.dv) acc[warp][g * 32 + lane] = x[g];
-  if (lane == 0) ml[warp] = make_float2(m, l);
-  __syncthreads();
-  float M = -CUDART_INF_F, sum = 0.f, f[4];
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[w].x);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[w].x);
+    for (int w = 0; w < 4; ++w) {
+      f[w] = ml[w].x == -CUDART_INF_F ? 0.f : ex2((ml[w].x - M) * kLog2e);
+      sum = fmaf(ml[w].y, f[w], sum);
+    }
+    Segment s;
+    s.tok0 = rec.tok0; s.row0 = rec.row0; s.g = rec.g;
+    const int64_t row = out_row(a, s, r);
+    for (int d = threadIdx.x; d < a.dv; d += 128) {
+      float v = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    f[w] = ml[w].x == -CUDART_INF_F ? 0.f : ex2((ml[w].x - M) * kLog2e);
-    sum = fmaf(ml[w].y, f[w], sum);
-  }
-  Segment s;
-  s.tok0 = rec.tok0; s.row0 = rec.row0; s.g = rec.g;
-  const int64_t row = out_row(a, s, r);
-  for (int d = threadIdx.x; d < a.dv; d += 128) {
-    float v = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) v = fmaf(acc[w][d], f[w], v);
-    Elem<T>::st((T*)a.out + row * a.dv + d, sum > 0.f ? v / sum : v);
-  }
-  if (threadIdx.x == 0) {
-    a.M[row] = M;
-    a.L[row] = logf(sum);
+      for (int w = 0; w < 4; ++w) v = fmaf(acc[w][d], f[w], v);
+      Elem<T>::st((T*)a.out + row * a.dv + d, sum > 0.f ? v / sum : v);
+    }
+    if (threadIdx.x == 0) {
+      a.M[row] = M;
+      a.L[row] = logf(sum);
+    }
   }
 }
 
 int launch_combine(const Cache4Args& a, int blocks, int rows, bool f32, cudaStream_t st) {
   KernelTimer kt("cache4_combine", st);
-  const dim3 grid(blocks, rows);
+  const dim3 grid(blocks, std::min(rows, kCombineRows));
   if (f32) cache4_combine_kernel<float><<<grid, 128, 0, st>>>(a, blocks, rows);
   else cache4_combine_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(a, blocks, rows);
   return check_launch("cache4_combine");
 }
 
-int cache4_sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-  return n;
-}
-
 // ------------------------------------------------------------------------------------------------ host side
 constexpr int kFmaRows = 8;
 constexpr int kC4Smem = 227 * 1024 - 4096;
+
+// rows (new tokens times heads of a group) from which a request goes to the tensor-memory kernel
+constexpr int kChunkRows = 128;
 
 static size_t ring_bytes(int dk, int dv) { return (size_t)kC4Warps * kC4Stages * ((dk + dv) / kGroupDims) * kRecBytesPerGroup; }
 
@@ -614,7 +609,9 @@ extern "C" NSA_API size_t nsa_cache4_attn_workspace_bytes(const nsa_cache4_desc*
   if (cache4_args(desc, a) != NSA_OK || a.N == 0 || a.S == 0) return 0;
   const int dtype = desc->dtype;
   const size_t fma = NSA_C4_FMA(core_workspace, a);
-  return mma_dims(a, dtype) ? std::max(fma, NSA_C4_MMA(core_workspace, a)) : fma;
+  if (!mma_dims(a, dtype)) return fma;
+  const size_t mma = NSA_C4_MMA(core_workspace, a);
+  return std::max({fma, mma, a.n_sel ? 0 : cache4_chunk_workspace(a)});
 }
 
 extern "C" NSA_API int nsa_cache4_attn_fwd(const nsa_cache4_desc* desc, void* workspace, size_t workspace_bytes, void* stream) {
@@ -630,6 +627,18 @@ extern "C" NSA_API int nsa_cache4_attn_fwd(const nsa_cache4_desc* desc, void* wo
   a.ws = (uint8_t*)workspace;
   cudaStream_t st = (cudaStream_t)stream;
   const int dtype = desc->dtype;
-  if (mma_dims(a, dtype) && mma_aligned(a)) return NSA_C4_MMA(launch_core, a, "cache4_attn_mma", st);
+  if (mma_dims(a, dtype) && mma_aligned(a)) {
+    // Each request goes to the kernel that suits its rows, by their numbers on the device; a launch that the host can tell to be empty is left out.
+    const int most = desc->max_new > 0 ? std::min(desc->max_new, a.N) : a.N;
+    const bool chunks = a.n_sel == 0 && (int64_t)most * a.hpg >= kChunkRows;
+    const bool uniform = desc->max_new > 0 && (int64_t)a.S * desc->max_new == a.N && chunks;
+    if (chunks) {
+      a.rows_lo = kChunkRows;
+      if (int rc = launch_chunk(a, st)) return rc;
+      a.rows_lo = 0;
+      a.rows_hi = kChunkRows;
+    }
+    return uniform ? NSA_OK : NSA_C4_MMA(launch_core, a, "cache4_attn_mma", st);
+  }
   return NSA_C4_FMA(launch_core, a, "cache4_attn_fma", st);
 }

@@ -31,7 +31,8 @@ struct SplitRecord {
 
 __device__ __forceinline__ long long share(long long total, int c, int n) { return total * c / n; }
 
-template <int ROWS>
+// KEYS: keys of a unit (one page, or two)
+template <int ROWS, int KEYS = kPageTokens>
 struct Walk {
   const Cache4Args& a;
   Segment s;
@@ -49,12 +50,12 @@ struct Walk {
     if (n * a.hpg < a.rows_lo || n * a.hpg >= a.rows_hi) n = 0;
     length = min(max(a.lengths[r], 0), 1 << 30);
   }
-  // pages that some row of tile t can see (at least one, so that every row is written)
-  __device__ __forceinline__ void pages(int length, int n, int t, int& lo, int& hi) const {
+  // units that some row of tile t can see (at least one, so that every row is written)
+  __device__ __forceinline__ void bounds(int length, int n, int t, int& lo, int& hi) const {
     const int p0 = length - n;
     const int first = p0 + t * ROWS / a.hpg, last = p0 + min(n * a.hpg - 1, t * ROWS + ROWS - 1) / a.hpg;
-    hi = last < 0 ? 0 : min(last / kPageTokens + 1, a.P);
-    lo = a.window > 0 ? max(first - a.window + 1, 0) / kPageTokens : 0;
+    hi = last < 0 ? 0 : min(last / KEYS + 1, (a.P * kPageTokens + KEYS - 1) / KEYS);
+    lo = a.window > 0 ? max(first - a.window + 1, 0) / KEYS : 0;
     if (hi <= lo) { lo = 0; hi = 1; }
   }
   __device__ __forceinline__ long long units(int r) const {
@@ -63,7 +64,7 @@ struct Walk {
     request(r, tok0, n, length);
     for (int t = 0, m = row_tiles(n); t < m; ++t) {
       int lo, hi;
-      pages(length, n, t, lo, hi);
+      bounds(length, n, t, lo, hi);
       sum += hi - lo;
     }
     return sum * a.G;
@@ -76,7 +77,7 @@ struct Walk {
       return;
     }
     s.nrows = min(ROWS, fresh * a.hpg - s.row0);
-    pages(len, fresh, tile, s.lo, s.hi);
+    bounds(len, fresh, tile, s.lo, s.hi);
   }
   __device__ __forceinline__ void set_request(int r) {
     s.r = r;
@@ -212,7 +213,10 @@ __device__ __forceinline__ int64_t out_row(const Cache4Args& a, const Segment& s
   return (int64_t)(s.tok0 + f / a.hpg) * a.H + s.g * a.hpg + f % a.hpg;
 }
 
+// the tensor-memory kernel for many rows a request (cache4_chunk.cu)
+size_t cache4_chunk_workspace(const Cache4Args& a);
+int launch_chunk(const Cache4Args& a, cudaStream_t st);
+
 int launch_combine(const Cache4Args& a, int blocks, int rows, bool f32, cudaStream_t st);
-int cache4_sm_count();
 
 }  // namespace nsa

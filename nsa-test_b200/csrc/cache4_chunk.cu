@@ -1,0 +1,583 @@
+// Chunks of many new tokens over the 4-bit paged cache on 5th-generation tensor cores (tcgen05 + TMEM).
+//
+// A block owns 256 rows (query token, head) of one kv group in two MMA tiles of 128 and walks the keys 128 at a time (two pages).  Roles (512 threads):
+//   warps 0-3 / 4-7  softmax of tile 0 / 1, one row per thread: they also bring the row's queries in (fp16, scaled to a largest magnitude
+//                    in [2^14, 2^15) by a power of two) and write its output
+//   warps 8-11       unpack a tile's keys and values out of L2 into shared memory: fp16 holds (c - 8) s exactly
+//   warp 13          walks the block's segments and hands the pieces to the others
+//   warp 12          issues the MMAs: S_i = Q_i K^T (both operands in shared memory), O_i += P_i V (P in tensor memory)
+// TMEM columns and the order PV0(j) QK0(j+1) PV1(j) QK1(j+1) are those of the dense forward kernel.  Probabilities are rounded to fp16 (2^-11).
+//
+// Where a code lies in its word fixes in which order a thread unpacks it for free; the two operands of a product only have to agree.  So
+// eight dimensions of a query and a key lie in the order 0 4 1 5 2 6 3 7, and dimension 8 e + n of a group of 32 values is column
+// 8 (n / 2) + 2 e + n % 2 of the output tile, put back in order when the row is written.
+//
+// Bound by the issue slots of the softmax (a multiply-add, an exponential, a maximum, half a conversion and an addition an element) and the
+// unpacking together, then by the tensor pipe: 2560 clocks a tile of 128 keys at head dims 192/128.
+#include <algorithm>
+
+#include "attn_args.cuh"
+#include "cache4_attn.cuh"
+#include "fa_sm100.cuh"
+#include "sm100_ptx.cuh"
+
+namespace nsa {
+
+using namespace ptx;
+
+constexpr int kChM = 128, kChN = 128, kChRows = 256, kChThreads = 512;
+constexpr int kChRegsSoftmax = 176, kChRegsUnpack = 104, kChRegsIssue = 56;
+constexpr int kChRegsNeeded = (256 * kChRegsSoftmax + 128 * kChRegsUnpack + 128 * kChRegsIssue + kChThreads - 1) / kChThreads;   // per thread at launch
+constexpr float kChGrow = 8.f;       // log2 units
+
+template <int DK, int DV>
+struct ChunkSmem {
+  static constexpr int kQBytes = kChM * DK * 2, kKBytes = kChN * DK * 2, kVBytes = kChN * DV * 2;
+  static constexpr int oQ = 0, oK = oQ + 2 * kQBytes, oV = oK + 2 * kKBytes, oBar = oV + kVBytes;
+  static constexpr int kDynamic = oBar + 768 + 1024;       // slack to align the base to the swizzle atom
+};
+
+// units [p0, p0 + n) of a segment, as one warp finds them and the roles take them; n = 0 ends the list
+struct ChunkPiece {
+  int tok0, row0, nrows, r, g, pos0, p0, n, whole, part;
+};
+constexpr int kChPieces = 4, kChRoleWarps = 13;
+
+struct ChunkBarriers {
+  uint64_t piece_full[kChPieces], piece_empty[kChPieces];
+  ChunkPiece piece[kChPieces];
+  uint64_t q_full[2], k_full[2], k_empty[2], v_full, v_empty, s_full[2], p_full[2], pv_done[2], o_free[2];
+  long long scratch[kChThreads / 32 + 3];
+  uint32_t tmem_base;
+  int abort;
+};
+
+// fp16 x fp16 -> fp32, dense
+constexpr uint32_t idesc_f16(int M, int N, int a_mn_major, int b_mn_major) {
+  return (1u << 4) | ((uint32_t)a_mn_major << 15) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+__device__ __forceinline__ uint32_t code_bits(uint32_t x, uint32_t mask) {      // (x & mask) | 1024 in both halves
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, 0x64006400, 0xEA;" : "=r"(r) : "r"(x), "r"(mask));
+  return r;
+}
+// 32 lanes x 8 consecutive 32-bit columns (the rescaling has few registers to spare beside a row's logits)
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+// four codes of each half of a word, nibble by nibble, times the half's scale
+__device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 s) {
+  const __half2 bias = __float2half2_rn(-1032.f), sixteenth = __float2half2_rn(0.0625f), bias16 = __float2half2_rn(-72.f);
+  const uint32_t v = w >> 8;
+  uint4 r;
+  r.x = h2u(__hmul2(__hadd2(u2h(code_bits(w, 0x000f000fu)), bias), s));
+  r.y = h2u(__hmul2(__hfma2(u2h(code_bits(w, 0x00f000f0u)), sixteenth, bias16), s));
+  r.z = h2u(__hmul2(__hadd2(u2h(code_bits(v, 0x000f000fu)), bias), s));
+  r.w = h2u(__hmul2(__hfma2(u2h(code_bits(v, 0x00f000f0u)), sixteenth, bias16), s));
+  return r;
+}
+
+template <int DK, int DV>
+__global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache4Args a, int* timeouts) {
+  using SM = ChunkSmem<DK, DV>;
+  constexpr int GK = DK / kGroupDims, GV = DV / kGroupDims, kRecBytes = (GK + GV) * kRecBytesPerGroup;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  ChunkBarriers* bar = reinterpret_cast<ChunkBarriers*>(smem + SM::oBar);
+  volatile int* abort = &bar->abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar->q_full[i], 128);
+      mbar_init(&bar->k_full[i], 128);
+      mbar_init(&bar->k_empty[i], 1);
+      mbar_init(&bar->s_full[i], 1);
+      mbar_init(&bar->p_full[i], 128);
+      mbar_init(&bar->pv_done[i], 1);
+      mbar_init(&bar->o_free[i], 128);
+    }
+    for (int i = 0; i < kChPieces; ++i) {
+      mbar_init(&bar->piece_full[i], 1);
+      mbar_init(&bar->piece_empty[i], kChRoleWarps);
+    }
+    mbar_init(&bar->v_full, 128);
+    mbar_init(&bar->v_empty, 1);
+    bar->abort = 0;
+    fence_barrier_init();
+    fence_proxy_async();
+  }
+  if (warp == 12) tmem_alloc(&bar->tmem_base, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bar->tmem_base;
+
+  Walk<kChRows, kChN> walk(a);
+  walk.template start<kChThreads>(bar->scratch);
+  // once any block has given up on a wait the device's results are void: later blocks skip their work
+  if (threadIdx.x == 0) bar->scratch[0] = *(volatile const int*)timeouts != 0 ? 0 : walk.total;
+  __syncthreads();
+  walk.total = bar->scratch[0];
+  __syncthreads();
+  const long long begin = share(walk.total, blockIdx.x, gridDim.x), end = share(walk.total, blockIdx.x + 1, gridDim.x);
+  const int place0 = begin < end ? walk.template seek<kChThreads>(begin, bar->scratch) : 0;
+  __syncthreads();
+  // piece number c of the block into registers, its place free again; a wait that runs out reads as the end of the list
+  auto take = [&](int c) {
+    ChunkPiece w;
+    if (mbar_wait_warp(&bar->piece_full[c % kChPieces], (c / kChPieces) & 1, abort)) {
+      w = bar->piece[c % kChPieces];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar->piece_empty[c % kChPieces]);
+    } else {
+      w.n = 0;
+    }
+    return w;
+  };
+  auto pages_of = [&](const ChunkPiece& w, int unit, int& id0, int& id1) {
+    id0 = 2 * unit < a.P ? a.table[w.r * a.table_ld + 2 * unit] : -1;
+    id1 = 2 * unit + 1 < a.P ? a.table[w.r * a.table_ld + 2 * unit + 1] : -1;
+    if (id0 >= a.n_pages) id0 = -1;
+    if (id1 >= a.n_pages) id1 = -1;
+  };
+
+  if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kChRegsIssue));
+    if (warp == 13) {
+      // ---------------------------------------------------------- the block's pieces
+      SplitRecord out{};
+      long long u = begin;
+      int place = place0;
+      for (int c = 0;; ++c) {
+        if (!mbar_wait_warp(&bar->piece_empty[c % kChPieces], ((c / kChPieces) & 1) ^ 1, abort)) break;
+        const Segment& s = walk.s;
+        ChunkPiece w{};
+        if (u < end) {
+          w = ChunkPiece{s.tok0, s.row0, s.nrows, s.r, s.g, s.pos0, s.lo + place, (int)min((long long)(s.hi - s.lo - place), end - u), 0, place == 0};
+          w.whole = place == 0 && w.n == s.hi - s.lo;
+          if (place == 0 && !w.whole) out = SplitRecord{1, s.tok0, s.row0, s.nrows, s.g, 0, u, u + s.hi - s.lo, walk.total};
+        }
+        if (lane == 0) {
+          bar->piece[c % kChPieces] = w;
+          mbar_arrive(&bar->piece_full[c % kChPieces]);
+        }
+        if (w.n == 0) break;
+        u += w.n;
+        place = 0;
+        if (u < end) walk.next();
+      }
+      if (lane == 0) reinterpret_cast<SplitRecord*>(a.ws)[blockIdx.x] = out;
+    } else if (warp == 12) {
+      // ---------------------------------------------------------- MMA issuer (warp-uniform loops, one elected lane issues)
+      constexpr uint32_t idQK = idesc_f16(kChM, kChN, 0, 0), idPV = idesc_f16(kChM, DV, 0, 1);
+      const uint64_t dQ0 = smem_desc_sw128(smem_u32(smem + SM::oQ), 16, 1024);
+      const uint64_t dK0 = smem_desc_sw128(smem_u32(smem + SM::oK), 16, 1024);
+      const uint64_t dV = smem_desc_sw128(smem_u32(smem + SM::oV), kChN * 128, 1024);
+      auto issue_qk = [&](int i, int ks) {
+        const uint64_t dQ = desc_advance(dQ0, i * SM::kQBytes), dK = desc_advance(dK0, ks * SM::kKBytes);
+#pragma unroll
+        for (int kk = 0; kk < DK / 16; ++kk)
+          umma_ss(tmem + i * 128, desc_advance(dQ, (kk >> 2) * (kChM * 128) + (kk & 3) * 32),
+                  desc_advance(dK, (kk >> 2) * (kChN * 128) + (kk & 3) * 32), idQK, kk > 0);
+        umma_commit(&bar->s_full[i]);
+      };
+      bool ok = true;
+      int kc = 0, ic0 = 0, ic1 = 0, sc0 = 0, sc1 = 0;     // key tiles; segments and key tiles of either MMA tile so far
+      for (int pc = 0; ok; ++pc) {
+        const ChunkPiece w = take(pc);
+        if (w.n == 0) break;
+        const bool two = w.nrows > kChM;
+        const int ntile = two ? 2 : 1;
+        ok = mbar_wait_warp(&bar->q_full[0], ic0 & 1, abort) && (!two || mbar_wait_warp(&bar->q_full[1], ic1 & 1, abort)) &&
+             mbar_wait_warp(&bar->k_full[kc & 1], (kc >> 1) & 1, abort);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          issue_qk(0, kc & 1);
+          if (two) issue_qk(1, kc & 1);
+          umma_commit(&bar->k_empty[kc & 1]);
+        }
+        __syncwarp();
+        for (int j = 0; j < w.n && ok; ++j, ++kc) {
+          const bool more = j + 1 < w.n;
+          ok = mbar_wait_warp(&bar->v_full, kc & 1, abort);
+          for (int i = 0; i < ntile && ok; ++i) {
+            ok = mbar_wait_warp(&bar->p_full[i], (i ? sc1 : sc0) & 1, abort);
+            if (ok && j == 0) ok = mbar_wait_warp(&bar->o_free[i], ((i ? ic1 : ic0) & 1) ^ 1, abort);
+            if (!ok) break;
+            const int ks = (kc + 1) & 1;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < kChN / 16; ++kk)
+                umma_ts(tmem + 256 + i * 128, tmem + i * 128 + kk * 8, desc_advance(dV, kk * 2048), idPV, (j > 0) || (kk > 0));
+              umma_commit(&bar->pv_done[i]);
+              if (i + 1 == ntile) umma_commit(&bar->v_empty);
+            }
+            __syncwarp();
+            if (more) {
+              if (i == 0) {
+                ok = mbar_wait_warp(&bar->k_full[ks], ((kc + 1) >> 1) & 1, abort);
+                if (!ok) break;
+                tc_fence_after();
+              }
+              if (elect_one()) {
+                issue_qk(i, ks);
+                if (i + 1 == ntile) umma_commit(&bar->k_empty[ks]);
+              }
+              __syncwarp();
+            }
+            if (i) ++sc1; else ++sc0;
+          }
+        }
+        ++ic0;
+        if (two) ++ic1;
+      }
+    }
+  } else if (warp >= 8) {
+    // ------------------------------------------------------------ keys and values: 4 bits in L2 -> fp16 in shared memory
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kChRegsUnpack));
+    const int wq = warp - 8, n = lane >> 2, j = lane & 3, first = 4 * (n >> 1) + (n & 1);
+    const int vg = lane >> 4, vu = (lane >> 2) & 3;
+    bool ok = true;
+    int kc = 0;
+    for (int pc = 0; ok; ++pc) {
+      const ChunkPiece s = take(pc);
+      if (s.n == 0) break;
+      const int maxpos = s.pos0 + (s.row0 + s.nrows - 1) / a.hpg;
+      const int minlow = a.window > 0 ? s.pos0 + s.row0 / a.hpg - a.window + 1 : 0;
+      for (int t = 0; t < s.n; ++t, ++kc) {
+        const int n0 = (s.p0 + t) * kChN;
+        int id0, id1;
+        pages_of(s, s.p0 + t, id0, id1);
+        const int id = wq < 2 ? id0 : id1;         // this warp's two records: half a page
+        const uint8_t* src = a.cache + (((int64_t)max(id, 0) * a.G + s.g) * kRecsPerPage + (wq & 1) * 2) * kRecBytes;
+        // keys: lane (n, j) holds 8 dimensions of tokens n and 8 + n; odd n take the odd group of a pair first, so that the eight
+        // lanes of a store phase fill all eight 16-byte columns
+        uint2 kw[2][GK];
+        __half kscale[2][GK][2];
+        if (id >= 0) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int g = 0; g < GK; ++g) {
+              const int gg = g ^ (n & 1);
+              const uint8_t* rec = src + r * kRecBytes;
+              kw[r][g] = __ldg(reinterpret_cast<const uint2*>(rec + gg * kChunkBytes + lane * 8));
+              const __half* sc = reinterpret_cast<const __half*>(rec + (GK + GV) * kChunkBytes + gg * kChunkScaleBytes) + first;
+              kscale[r][g][0] = __ldg(sc);
+              kscale[r][g][1] = __ldg(sc + 2);
+            }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int g = 0; g < GK; ++g) {
+              kw[r][g] = make_uint2(0, 0);
+              kscale[r][g][0] = kscale[r][g][1] = __ushort_as_half(0);
+            }
+        }
+        ok = mbar_wait_warp(&bar->k_empty[kc & 1], ((kc >> 1) & 1) ^ 1, abort);
+        if (!ok) break;
+        uint8_t* sK = smem + SM::oK + (kc & 1) * SM::kKBytes;
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int g = 0; g < GK; ++g) {
+            const int gg = g ^ (n & 1), row = (wq * 2 + r) * 16 + n;
+            uint8_t* dst = sK + (g >> 1) * (kChN * 128) + row * 128 + ((((gg & 1) * 4 + j) ^ n) << 4);
+            *reinterpret_cast<uint4*>(dst) = unpack8(kw[r][g].x, __half2half2(kscale[r][g][0]));
+            *reinterpret_cast<uint4*>(dst + 8 * 128) = unpack8(kw[r][g].y, __half2half2(kscale[r][g][1]));
+          }
+        fence_proxy_async();
+        mbar_arrive(&bar->k_full[kc & 1]);
+        // values: lane (group of a pair, dimensions n = 2 u and 2 u + 1, tokens 2 j, 2 j + 1, 8 + 2 j, 8 + 2 j + 1)
+        uint2 v0[2][GV / 2], v1[2][GV / 2], vs[2][GV / 2];
+        if (id >= 0) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int g = 0; g < GV / 2; ++g) {
+              const uint8_t* rec = src + r * kRecBytes;
+              const uint2* c = reinterpret_cast<const uint2*>(rec + (GK + 2 * g + vg) * kChunkBytes);
+              v0[r][g] = __ldg(c + 8 * vu + j);
+              v1[r][g] = __ldg(c + 8 * vu + 4 + j);
+              vs[r][g] = __ldg(reinterpret_cast<const uint2*>(rec + (GK + GV) * kChunkBytes + (GK + 2 * g + vg) * kChunkScaleBytes) + j);
+            }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int g = 0; g < GV / 2; ++g) v0[r][g] = v1[r][g] = vs[r][g] = make_uint2(0, 0);
+        }
+        // what no row sees may never have been written: nothing of it enters, not as 0 times it either
+        const bool edge = n0 + kChN - 1 > maxpos || n0 < minlow;
+        ok = mbar_wait_warp(&bar->v_empty, (kc & 1) ^ 1, abort);
+        if (!ok) break;
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int g = 0; g < GV / 2; ++g) {
+            uint8_t* dst = smem + SM::oV + g * (kChN * 128);
+            const int rec0 = (wq * 2 + r) * 16;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {             // token 8 (q / 2) + 2 j + q % 2
+              const int row = rec0 + 8 * (q >> 1) + 2 * j + (q & 1);
+              const uint32_t x = q < 2 ? v0[r][g].x : v0[r][g].y, y = q < 2 ? v1[r][g].x : v1[r][g].y, z = q < 2 ? vs[r][g].x : vs[r][g].y;
+              uint32_t sc = __byte_perm(z, z, q & 1 ? 0x3232 : 0x1010);
+              if (edge && (n0 + row > maxpos || n0 + row < minlow)) sc = 0;
+              *reinterpret_cast<uint4*>(dst + row * 128 + (((vg * 4 + vu) ^ (row & 7)) << 4)) =
+                  unpack8(__byte_perm(x, y, q & 1 ? 0x7632 : 0x5410), u2h(sc));
+            }
+          }
+        fence_proxy_async();
+        mbar_arrive(&bar->v_full);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax and epilogue, one row per thread
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kChRegsSoftmax));
+    const int i = warp >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lane_base + i * 128, tO = tmem + lane_base + 256 + i * 128;
+    float cl = 0.f;                      // logit of a unit of S
+    int pos = -1;
+    // this thread's row of the current segment into shared memory, as far as the segment has one
+    auto load_q = [&](const ChunkPiece& s) {
+      const int row = i * kChM + r, f = s.row0 + row;
+      const bool there = row < s.nrows;
+      pos = there ? s.pos0 + f / a.hpg : -1;
+      uint4 raw[DK / 8];
+      const uint4* src = reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + (s.tok0 + f / a.hpg) * a.sq_tok + (s.g * a.hpg + f % a.hpg) * a.sq_head);
+      uint32_t mx = 0;
+#pragma unroll
+      for (int c = 0; c < DK / 8; ++c) {
+        raw[c] = there ? src[c] : make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = max(mx, max(w[e] & 0x7fffu, w[e] >> 16 & 0x7fffu));
+      }
+      const int k = mx ? min(14 - ((int)(mx >> 7) - 127), 100) : 0;
+      // the scale's sign goes into the row, so that larger S is always the larger logit; scale 0 is a row of zeros
+      const float up = __uint_as_float((uint32_t)(k + 127) << 23) * (a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f);
+      cl = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * __uint_as_float((uint32_t)(127 - k) << 23);
+      uint8_t* dst = smem + SM::oQ + i * SM::kQBytes + r * 128;
+#pragma unroll
+      for (int c = 0; c < DK / 8; ++c) {
+        const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[2 * e] = __uint_as_float(w[e] << 16) * up;
+          x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u) * up;
+        }
+        uint4 o;
+        o.x = h2u(__floats2half2_rn(x[0], x[4]));
+        o.y = h2u(__floats2half2_rn(x[1], x[5]));
+        o.z = h2u(__floats2half2_rn(x[2], x[6]));
+        o.w = h2u(__floats2half2_rn(x[3], x[7]));
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * (kChM * 128) + (((c & 7) ^ (r & 7)) << 4)) = o;
+      }
+      fence_proxy_async();
+      mbar_arrive(&bar->q_full[i]);
+    };
+    bool ok = true;
+    int sc = 0;                          // key tiles of earlier segments (barrier phases run on)
+    int pc = 0;
+    auto take_rows = [&]() {             // the next piece that has rows for this tile
+      ChunkPiece w;
+      do w = take(pc++); while (w.n > 0 && i * kChM >= w.nrows);
+      return w;
+    };
+    ChunkPiece s = take_rows();
+    if (s.n > 0) load_q(s);
+    while (s.n > 0) {
+      const int row0 = s.row0 + i * kChM, my_pos = pos;
+      const float c2 = cl * kLog2e, thr = kChGrow / c2, row_cl = cl;
+      const int minpos = s.pos0 + row0 / a.hpg, maxpos = s.pos0 + (s.row0 + min(s.nrows, (i + 1) * kChM) - 1) / a.hpg;
+      float m_true = -CUDART_INF_F, m_ref = -CUDART_INF_F, l = 0.f;
+      int id0, id1;
+      pages_of(s, s.p0, id0, id1);
+      for (int t = 0; t < s.n && ok; ++t) {
+        const int n0 = (s.p0 + t) * kChN, c0 = id0, c1 = id1;
+        if (t + 1 < s.n) pages_of(s, s.p0 + t + 1, id0, id1);
+        ok = mbar_wait_warp(&bar->s_full[i], (sc + t) & 1, abort);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t sv[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, sv[c]);
+        tc_wait_ld();
+        const bool full = c0 >= 0 && c1 >= 0 && n0 + kChN - 1 <= minpos && (a.window == 0 || n0 > maxpos - a.window);
+        if (!full) {
+          int clo = a.window > 0 ? my_pos - a.window - n0 : -1, chi = my_pos - n0;       // visible columns: clo < c <= chi
+          if (c0 < 0) clo = max(clo, kPageTokens - 1);
+          if (c1 < 0) chi = min(chi, kPageTokens - 1);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (c * 32 + e <= clo || c * 32 + e > chi) sv[c][e] = 0xff800000u;
+        }
+        float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(sv[c][e]));
+        m_true = fmaxf(m_true, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+        const bool first = m_ref == -CUDART_INF_F;
+        const bool grow = first ? m_true > m_ref : m_true > m_ref + thr;
+        const bool need_o = grow && !first;
+        if (__any_sync(0xffffffffu, need_o)) {
+          ok = mbar_wait_warp(&bar->pv_done[i], (sc + t - 1) & 1, abort);   // O_i must hold PV(t - 1) before it is scaled
+          if (!ok) break;
+          tc_fence_after();
+          const float f = need_o ? ex2((m_ref - m_true) * c2) : 1.f;
+          l *= f;
+#pragma unroll 2
+          for (int c = 0; c < DV / 8; ++c) {
+            uint32_t ov[8];
+            tmem_ld8(tO + c * 8, ov);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * f);
+            tmem_st8(tO + c * 8, ov);
+          }
+          tc_wait_st();
+        }
+        if (grow) m_ref = m_true;
+        const float mb = m_ref == -CUDART_INF_F ? 0.f : -m_ref * c2;
+        float rs[2] = {0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; c += 2) {          // probabilities take the places of the logits they come from
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int cc = c + (e >> 4), ee = (e & 15) * 2;
+            const float p0 = ex2(fmaf(__uint_as_float(sv[cc][ee]), c2, mb)), p1 = ex2(fmaf(__uint_as_float(sv[cc][ee + 1]), c2, mb));
+            rs[0] += p0;
+            rs[1] += p1;
+            sv[c][e] = h2u(__floats2half2_rn(p0, p1));
+          }
+          tmem_st32(tS + c * 16, sv[c]);
+        }
+        l += rs[0] + rs[1];
+        tc_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bar->p_full[i]);
+      }
+      if (!ok) break;
+      const int last = (sc + s.n - 1) & 1;
+      sc += s.n;
+      // the next piece of this tile: its queries go in while the last products run (its S has been read, so Q is free)
+      const ChunkPiece next = take_rows();
+      if (next.n > 0) load_q(next);
+      ok = mbar_wait_warp(&bar->pv_done[i], last, abort);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t ov[GV][32];
+#pragma unroll
+      for (int c = 0; c < GV; ++c) tmem_ld32(tO + c * 32, ov[c]);
+      tc_wait_ld();
+      tc_fence_before();
+      mbar_arrive(&bar->o_free[i]);
+      const int row = i * kChM + r;
+      if (row < s.nrows) {
+        const float rel = l > 0.f ? ex2((m_ref - m_true) * c2) : 1.f;       // results relative to the row's true maximum
+        const float f = s.whole ? (l > 0.f ? 1.f / l : 1.f) : rel;
+        float* part = s.whole ? nullptr : split_part(a, gridDim.x, kChRows, blockIdx.x, s.part);
+        Segment sg;
+        sg.tok0 = s.tok0; sg.row0 = s.row0; sg.g = s.g;
+        const int64_t orow = out_row(a, sg, row);
+#pragma unroll
+        for (int g = 0; g < GV; ++g)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x[8];                                                     // dimensions 8 e + 0..7: columns 8 (n / 2) + 2 e + n % 2
+#pragma unroll
+            for (int n = 0; n < 8; ++n) x[n] = __uint_as_float(ov[g][8 * (n >> 1) + 2 * e + (n & 1)]) * f;
+            if (s.whole) {
+              uint4 pkt;
+              __nv_bfloat162 b[4];
+#pragma unroll
+              for (int n = 0; n < 4; ++n) b[n] = __floats2bfloat162_rn(x[2 * n], x[2 * n + 1]);
+              pkt.x = *reinterpret_cast<uint32_t*>(&b[0]);
+              pkt.y = *reinterpret_cast<uint32_t*>(&b[1]);
+              pkt.z = *reinterpret_cast<uint32_t*>(&b[2]);
+              pkt.w = *reinterpret_cast<uint32_t*>(&b[3]);
+              *reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + orow * DV + g * 32 + e * 8) = pkt;
+            } else {
+              float4* to = reinterpret_cast<float4*>(part + row * DV + g * 32 + e * 8);
+              to[0] = make_float4(x[0], x[1], x[2], x[3]);
+              to[1] = make_float4(x[4], x[5], x[6], x[7]);
+            }
+          }
+        const float M = m_true == -CUDART_INF_F ? m_true : m_true * row_cl;
+        if (s.whole) {
+          a.M[orow] = M;
+          a.L[orow] = logf(l * rel);
+        } else {
+          reinterpret_cast<float2*>(part + kChRows * DV)[row] = make_float2(M, l * rel);
+        }
+      }
+      s = next;
+    }
+  }
+
+  // ------------------------------------------------------------ teardown (every thread gets here)
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && bar->abort) report_timeout(timeouts);
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+static int chunk_blocks() { return 148; }
+
+size_t cache4_chunk_workspace(const Cache4Args& a) { return split_bytes(chunk_blocks(), kChRows, a.dv); }
+
+template <int DK, int DV>
+static int launch_chunk_t(const Cache4Args& a, cudaStream_t st) {
+  using SM = ChunkSmem<DK, DV>;
+  auto kern = cache4_chunk_kernel<DK, DV>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::kDynamic);
+  if (e != cudaSuccess) return fail(NSA_ERR_LAUNCH, "cache4_chunk: cannot reserve %d bytes of shared memory: %s", SM::kDynamic, cudaGetErrorString(e));
+  // the split of registers over the roles draws on what the block is launched with
+  cudaFuncAttributes at;
+  e = cudaFuncGetAttributes(&at, kern);
+  if (e != cudaSuccess || at.numRegs < kChRegsNeeded)
+    return fail(NSA_ERR_LAUNCH, "cache4_chunk: built with %d registers a thread, the roles share %d", at.numRegs, kChRegsNeeded);
+  int* timeouts = fa_timeout_counter();
+  if (!timeouts) return fail(NSA_ERR_LAUNCH, "cache4_chunk: cannot set up the time-out record of this device");
+  {
+    KernelTimer kt("cache4_chunk", st);
+    kern<<<chunk_blocks(), kChThreads, SM::kDynamic, st>>>(a, timeouts);
+    if (int rc = check_launch("cache4_chunk")) return rc;
+  }
+  return launch_combine(a, chunk_blocks(), kChRows, false, st);
+}
+
+int launch_chunk(const Cache4Args& a, cudaStream_t st) {
+  if (timeout_flagged())
+    return fail(NSA_ERR_LAUNCH, "cache4_attn: a tensor-core kernel gave up on a barrier wait earlier (device time-out); results since then are "
+                "invalid.  nsa_device_timeouts(1) reports and clears the condition");
+  if (a.dk == 192 && a.dv == 128) return launch_chunk_t<192, 128>(a, st);
+  if (a.dk == 128 && a.dv == 128) return launch_chunk_t<128, 128>(a, st);
+  if (a.dk == 64 && a.dv == 64) return launch_chunk_t<64, 64>(a, st);
+  return fail(NSA_ERR_UNSUPPORTED, "cache4_chunk: unsupported head dims");
+}
+
+}  // namespace nsa
