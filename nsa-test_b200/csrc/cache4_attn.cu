@@ -147,217 +147,6 @@ struct FmaCore {
 };
 
 // ------------------------------------------------------------------------------------------------
-// bf16 queries on mma.m16n8k16 with fp16 operands and 32-bit sums, 16 rows a tile, a record of 16 keys at a time per warp.
-//
-// Logits: a nibble c masked out of its word where it lies is the fp16 number c 2^-24 (or 16 c 2^-24: subnormal numbers are multiples of 2^-24,
-// and their bits are the multiple), so unpacking costs one AND per two codes; the sums start from -8 sum(q) 2^-24, which turns codes into
-// values.  Each 32 dimensions are multiplied by their scale in 32 bits.  Queries are scaled to a largest magnitude in [2^14, 2^15)
-// per row (a power of two; bf16 has 8 bits, fp16 11, so only elements 2^-20 below the row's largest lose any) and the two pairs whose codes
-// arrive 16 times too large are divided by 16.  All of it is exact but for the 32-bit sums.
-// Outputs: values times scales are exact in fp16; probabilities are rounded to fp16 (2^-11, an eighth of the output's own rounding).
-// The reference maximum moves only when a row's maximum outgrows it by a factor of 245, so probabilities stay far below 65504.
-// ------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-// (x & mask) | bits in one instruction
-__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
-  return r;
-}
-
-template <int GK, int GV>
-struct MmaCore {
-  static constexpr int kRows = 16, kBlocksPerSm = GV > 2 ? 3 : 5;
-  static constexpr float kGrow = 5.5f;
-  uint32_t q[GK][2][4];
-  float c0[GK][2];              // -8 sum(q) 2^-24 of rows n, n + 8
-  float o[GV][4][4];
-  float m[2], top[2], l[2], cl[2];
-  int pos[2];
-
-  static size_t extra_smem(int) { return 0; }
-
-  __device__ __forceinline__ void begin(const Cache4Args& a, const Segment& s, uint8_t*) {
-    const int lane = threadIdx.x & 31, n = lane >> 2, j = lane & 3;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int i = n + 8 * h, f = s.row0 + i;
-      const bool row = i < s.nrows;
-      pos[h] = row ? s.pos0 + f / a.hpg : -1;
-      uint4 raw[GK];
-      const __nv_bfloat16* src = (const __nv_bfloat16*)a.q + (s.tok0 + f / a.hpg) * a.sq_tok + (s.g * a.hpg + f % a.hpg) * a.sq_head + 8 * j;
-      uint32_t mx = 0;
-#pragma unroll
-      for (int g = 0; g < GK; ++g) {
-        raw[g] = row ? *reinterpret_cast<const uint4*>(src + g * kGroupDims) : make_uint4(0, 0, 0, 0);
-        const uint32_t u[4] = {raw[g].x, raw[g].y, raw[g].z, raw[g].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx = max(mx, max(u[e] & 0x7fffu, u[e] >> 16 & 0x7fffu));
-      }
-      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const int k = mx ? min(14 - ((int)(mx >> 7) - 127), 100) : 0;
-      const float up = __uint_as_float((uint32_t)(min(k, 100) + 127) << 23);
-      cl[h] = a.scale * __uint_as_float((uint32_t)(127 - k) << 23);
-#pragma unroll
-      for (int g = 0; g < GK; ++g) {
-        const uint32_t u[4] = {raw[g].x, raw[g].y, raw[g].z, raw[g].w};
-        float x[8], sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[2 * e] = __uint_as_float(u[e] << 16) * up;
-          x[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u) * up;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {                                 // dimensions e and e + 4: nibbles e, e + 4
-          const float w = e & 1 ? 0.0625f : 1.f;
-          const __half2 p = __floats2half2_rn(x[e] * w, x[e + 4] * w);
-          sum += (__low2float(p) + __high2float(p)) * (e & 1 ? 16.f : 1.f);
-          q[g][e >> 1][2 * (e & 1) + h] = as_u32(p);
-        }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        c0[g][h] = sum * -4.76837158203125e-07f;                      // 8 * 2^-24
-      }
-      m[h] = top[h] = -CUDART_INF_F;
-      l[h] = 0.f;
-    }
-#pragma unroll
-    for (int g = 0; g < GV; ++g)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[g][e][i] = 0.f;
-  }
-
-  __device__ __forceinline__ void record(const Cache4Args& a, const Segment& s, const uint8_t* rec, int base, int maxpos, int minlow) {
-    const int lane = threadIdx.x & 31, j = lane & 3;
-    const uint8_t* scales = rec + (GK + GV) * kChunkBytes + j * 8;
-    float x[2][4];                  // [tile of 8 keys][row n: keys 2 j, 2 j + 1; row n + 8: the same]
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i >> 2][i & 3] = 0.f;
-#pragma unroll
-    for (int g = 0; g < GK; ++g) {
-      const uint2 w = *reinterpret_cast<const uint2*>(rec + g * kChunkBytes + lane * 8);
-      const uint2 sc = *reinterpret_cast<const uint2*>(scales + g * kChunkScaleBytes);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint32_t u = t ? w.y : w.x, v = u >> 8;
-        float c[4] = {c0[g][0], c0[g][0], c0[g][1], c0[g][1]};
-        mma16816(c, q[g][0], u & 0x000f000fu, u & 0x00f000f0u);
-        mma16816(c, q[g][1], v & 0x000f000fu, v & 0x00f000f0u);
-        const float2 f = __half22float2(as_half2(t ? sc.y : sc.x));
-        x[t][0] = fmaf(c[0], f.x, x[t][0]);
-        x[t][1] = fmaf(c[1], f.y, x[t][1]);
-        x[t][2] = fmaf(c[2], f.x, x[t][2]);
-        x[t][3] = fmaf(c[3], f.y, x[t][3]);
-      }
-    }
-    const bool partial = base + kRecTokens - 1 > s.pos0 + s.row0 / a.hpg || (a.window > 0 && base <= maxpos - a.window);
-    float mx[2] = {-CUDART_INF_F, -CUDART_INF_F};
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[t][i] = x[t][i] * 16777216.f * cl[i >> 1];
-        if (partial) {
-          const int at = base + 8 * t + 2 * j + (i & 1), p = pos[i >> 1];
-          if (at > p || (a.window > 0 && at <= p - a.window)) x[t][i] = -CUDART_INF_F;
-        }
-        mx[i >> 1] = fmaxf(mx[i >> 1], x[t][i]);
-      }
-    top[0] = fmaxf(top[0], mx[0]);
-    top[1] = fmaxf(top[1], mx[1]);
-    if (__any_sync(0xffffffffu, mx[0] > m[0] + kGrow || mx[1] > m[1] + kGrow)) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float w = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-        w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, 2));
-        if (w > m[h] + kGrow) {
-          const float f = ex2((m[h] - w) * kLog2e);
-          m[h] = w;
-          l[h] *= f;
-#pragma unroll
-          for (int g = 0; g < GV; ++g)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              o[g][e][2 * h] *= f;
-              o[g][e][2 * h + 1] *= f;
-            }
-        }
-      }
-    }
-    const float b0 = m[0] == -CUDART_INF_F ? 0.f : m[0] * -kLog2e, b1 = m[1] == -CUDART_INF_F ? 0.f : m[1] * -kLog2e;
-    uint32_t p[4];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const float p0 = ex2(fmaf(x[t][0], kLog2e, b0)), p1 = ex2(fmaf(x[t][1], kLog2e, b0));
-      const float p2 = ex2(fmaf(x[t][2], kLog2e, b1)), p3 = ex2(fmaf(x[t][3], kLog2e, b1));
-      l[0] += p0 + p1;
-      l[1] += p2 + p3;
-      p[2 * t] = as_u32(__floats2half2_rn(p0, p1));
-      p[2 * t + 1] = as_u32(__floats2half2_rn(p2, p3));
-    }
-    // what no row sees may never have been written: nothing of it enters, not as 0 times it either
-    uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-    if (base + kRecTokens - 1 > maxpos || base < minlow) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int at = base + 8 * t + 2 * j;
-        keep[t] = (at <= maxpos && at >= minlow ? 0xffffu : 0u) | (at + 1 <= maxpos && at + 1 >= minlow ? 0xffff0000u : 0u);
-      }
-    }
-    const __half2 bias = __float2half2_rn(-1032.f), sixteenth = __float2half2_rn(0.0625f), bias16 = __float2half2_rn(-72.f);
-#pragma unroll
-    for (int g = 0; g < GV; ++g) {
-      const uint2 w = *reinterpret_cast<const uint2*>(rec + (GK + g) * kChunkBytes + lane * 8);
-      const uint2 sc = *reinterpret_cast<const uint2*>(scales + (GK + g) * kChunkScaleBytes);
-      const __half2 s0 = as_half2(sc.x & keep[0]), s1 = as_half2(sc.y & keep[1]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t u0 = e < 2 ? w.x : w.x >> 8, u1 = e < 2 ? w.y : w.y >> 8;
-        __half2 v0, v1;                                    // 1024 + c, or 1024 + 16 c: to c - 8, then times the scale
-        if (e & 1) {
-          v0 = __hfma2(as_half2(and_or(u0, 0x00f000f0u, 0x64006400u)), sixteenth, bias16);
-          v1 = __hfma2(as_half2(and_or(u1, 0x00f000f0u, 0x64006400u)), sixteenth, bias16);
-        } else {
-          v0 = __hadd2(as_half2(and_or(u0, 0x000f000fu, 0x64006400u)), bias);
-          v1 = __hadd2(as_half2(and_or(u1, 0x000f000fu, 0x64006400u)), bias);
-        }
-        mma16816(o[g][e], p, as_u32(__hmul2(v0, s0)), as_u32(__hmul2(v1, s1)));
-      }
-    }
-  }
-
-  __device__ __forceinline__ void finish(const Cache4Args& a, float* so, float2* ml) {
-    const int lane = threadIdx.x & 31, n = lane >> 2, j = lane & 3;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float t = top[h], sum = l[h];
-#pragma unroll
-      for (int d = 1; d < 4; d <<= 1) {
-        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
-        sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      }
-      // results relative to the row's true maximum
-      const float f = t == -CUDART_INF_F ? 0.f : ex2((m[h] - t) * kLog2e);
-      if (j == 0) ml[n + 8 * h] = make_float2(t, sum * f);
-#pragma unroll
-      for (int g = 0; g < GV; ++g)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          *reinterpret_cast<float2*>(so + (n + 8 * h) * (GV * 32) + g * 32 + e * 8 + 2 * j) = make_float2(o[g][e][2 * h] * f, o[g][e][2 * h + 1] * f);
-    }
-  }
-};
-
-// ------------------------------------------------------------------------------------------------
 template <typename T, class Core>
 __global__ void __launch_bounds__(kC4Threads, Core::kBlocksPerSm) cache4_attn_kernel(const Cache4Args a) {
   constexpr int ROWS = Core::kRows;
@@ -453,80 +242,121 @@ __global__ void __launch_bounds__(kC4Threads, Core::kBlocksPerSm) cache4_attn_ke
         if (d == 0) reinterpret_cast<float2*>(part + ROWS * a.dv)[r] = make_float2(m, l);
       }
     }
-    if (!whole && place == 0) out = SplitRecord{1, s.tok0, s.row0, s.nrows, s.g, 0, u, u + s.hi - s.lo, walk.total};
+    if (!whole && place == 0)
+      out = SplitRecord{block_of(walk.total, u + s.hi - s.lo - 1, gridDim.x) - (int)blockIdx.x + 1, s.tok0, s.row0, s.nrows, s.g, {}};
     u += n;
     place = 0;
     __syncthreads();
     if (u < end) walk.next();
   }
   if (threadIdx.x == 0) reinterpret_cast<SplitRecord*>(a.ws)[blockIdx.x] = out;
+  pdl_launch();
 }
 
-// Joins the partial results of the rows of one split segment: block (owner, first row).  The pieces are the owner's last segment and the
-// first segments of the blocks after it; four warps take every fourth of them, in a fixed order.
-constexpr int kCombineRows = 32;           // rows of an owner at once
-template <typename T>
+// Joins the partial results of a split segment's rows.  The pieces are the owner's last segment and the first segments of the blocks
+// after it.  WARPS = 4: a block has one row and its warps share the pieces (few rows, possibly hundreds of pieces); 1: a warp has a row
+// (the many rows of a chunk, whose segments fall into two or three pieces).  Weights first, 32 pieces at a time with a lane each, then the
+// weighted sum, whose loads do not depend on one another; the order is fixed.
+template <typename T, int WARPS>
 __global__ void __launch_bounds__(128) cache4_combine_kernel(const Cache4Args a, int blocks, int rows) {
+  pdl_wait();
   const SplitRecord rec = reinterpret_cast<const SplitRecord*>(a.ws)[blockIdx.x];
-  if (!rec.open || (int)blockIdx.y >= rec.nrows) return;
-  __shared__ float acc[4][kMaxHeadDim];
-  __shared__ float2 ml[4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int last = blockIdx.x;                   // the last block that has a unit of the segment
-  for (int up = blocks; up - last > 1;) {
-    const int mid = (last + up) >> 1;
-    if (share(rec.total, mid, blocks) < rec.last) last = mid; else up = mid;
-  }
-  for (int r = blockIdx.y; r < rec.nrows; r += kCombineRows) {
-    float m = -CUDART_INF_F, l = 0.f, x[kMaxHeadDim / 32] = {};
-    for (int c = blockIdx.x + warp; c <= last; c += 4) {
-      if (c > (int)blockIdx.x && share(rec.total, c, blocks) == share(rec.total, c + 1, blocks)) continue;   // more blocks than units
-      const float* part = split_part(a, blocks, rows, c, c == (int)blockIdx.x ? 1 : 0);
-      const float2 h = reinterpret_cast<const float2*>(part + rows * a.dv)[r];
-      if (h.x == -CUDART_INF_F) continue;
-      const float mx = fmaxf(m, h.x), f0 = m == -CUDART_INF_F ? 0.f : ex2((m - mx) * kLog2e), f1 = ex2((h.x - mx) * kLog2e);
-      m = mx;
-      l = l * f0 + h.y * f1;
+  const int r = WARPS == 4 ? blockIdx.y : blockIdx.y * 4 + warp;
+  if (rec.pieces == 0 || (WARPS == 4 ? (int)blockIdx.y : (int)blockIdx.y * 4) >= rec.nrows) return;
+  if (WARPS == 1 && r >= rec.nrows) return;
+  __shared__ float acc[WARPS == 4 ? 4 : 1][kMaxHeadDim];
+  __shared__ float2 ml[4];
+  const int q0 = WARPS == 4 ? warp : 0;                   // this warp's pieces: q0, q0 + WARPS, ...
+  const float* first = split_part(a, blocks, rows, blockIdx.x, 1);
+  const float* others = split_part(a, blocks, rows, blockIdx.x, 0);
+  const size_t step = 2 * split_part_floats(rows, a.dv);
+  auto part = [&](int p) { return p == 0 ? first : others + (size_t)p * step; };
+  float m = -CUDART_INF_F, l = 0.f;
+  float4 x[2] = {};                                       // dimensions 4 lane + 128 i
+  for (int p0 = q0; p0 < rec.pieces; p0 += 32 * WARPS) {
+    const int p = p0 + lane * WARPS;
+    float2 h = make_float2(-CUDART_INF_F, 0.f);
+    if (p < rec.pieces) h = reinterpret_cast<const float2*>(part(p) + rows * a.dv)[r];
+    const float mx = fmaxf(m, warp_max(h.x));
+    if (mx == -CUDART_INF_F) continue;
+    const float f = ex2((m - mx) * kLog2e), w = ex2((h.x - mx) * kLog2e);
+    m = mx;
+    l = l * f + warp_sum(h.y * w);
 #pragma unroll
-      for (int g = 0; g < kMaxHeadDim / 32; ++g)
-        if (g * 32 < a.dv) x[g] = x[g] * f0 + part[r * a.dv + g * 32 + lane] * f1;
+    for (int i = 0; i < 2; ++i) { x[i].x *= f; x[i].y *= f; x[i].z *= f; x[i].w *= f; }
+    const int n = min(32, (rec.pieces - p0 + WARPS - 1) / WARPS);
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+      const float wk = __shfl_sync(0xffffffffu, w, k);
+      const float4* src = reinterpret_cast<const float4*>(part(p0 + k * WARPS) + r * a.dv);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (lane * 4 + i * 128 < a.dv) {
+          const float4 v = src[lane + i * 32];
+          x[i].x = fmaf(v.x, wk, x[i].x); x[i].y = fmaf(v.y, wk, x[i].y); x[i].z = fmaf(v.z, wk, x[i].z); x[i].w = fmaf(v.w, wk, x[i].w);
+        }
     }
-    __syncthreads();
+  }
+  Segment s;
+  s.tok0 = rec.tok0; s.row0 = rec.row0; s.g = rec.g;
+  const int64_t row = out_row(a, s, r);
+  float f[4] = {1.f, 0.f, 0.f, 0.f};
+  if (WARPS == 4) {
 #pragma unroll
-    for (int g = 0; g < kMaxHeadDim / 32; ++g)
-      if (g * 32 < a.dv) acc[warp][g * 32 + lane] = x[g];
+    for (int i = 0; i < 2; ++i)
+      if (lane * 4 + i * 128 < a.dv) *reinterpret_cast<float4*>(&acc[warp][lane * 4 + i * 128]) = x[i];
     if (lane == 0) ml[warp] = make_float2(m, l);
     __syncthreads();
-    float M = -CUDART_INF_F, sum = 0.f, f[4];
-#pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[w].x);
+    if (warp > 0) return;
+    m = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
+    l = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      f[w] = ml[w].x == -CUDART_INF_F ? 0.f : ex2((ml[w].x - M) * kLog2e);
-      sum = fmaf(ml[w].y, f[w], sum);
+      f[w] = ml[w].x == -CUDART_INF_F ? 0.f : ex2((ml[w].x - m) * kLog2e);
+      l = fmaf(ml[w].y, f[w], l);
     }
-    Segment s;
-    s.tok0 = rec.tok0; s.row0 = rec.row0; s.g = rec.g;
-    const int64_t row = out_row(a, s, r);
-    for (int d = threadIdx.x; d < a.dv; d += 128) {
-      float v = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) v = fmaf(acc[w][d], f[w], v);
-      Elem<T>::st((T*)a.out + row * a.dv + d, sum > 0.f ? v / sum : v);
+    for (int i = 0; i < 2; ++i)
+      if (lane * 4 + i * 128 < a.dv) {
+        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float4 v = *reinterpret_cast<const float4*>(&acc[w][lane * 4 + i * 128]);
+          x[i].x = fmaf(v.x, f[w], x[i].x); x[i].y = fmaf(v.y, f[w], x[i].y); x[i].z = fmaf(v.z, f[w], x[i].z); x[i].w = fmaf(v.w, f[w], x[i].w);
+        }
+      }
+  }
+  const float inv = l > 0.f ? 1.f / l : 1.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (lane * 4 + i * 128 < a.dv) {
+      T* to = (T*)a.out + row * a.dv + lane * 4 + i * 128;
+      Elem<T>::st(to, x[i].x * inv); Elem<T>::st(to + 1, x[i].y * inv); Elem<T>::st(to + 2, x[i].z * inv); Elem<T>::st(to + 3, x[i].w * inv);
     }
-    if (threadIdx.x == 0) {
-      a.M[row] = M;
-      a.L[row] = logf(sum);
-    }
+  if (lane == 0) {
+    a.M[row] = m;
+    a.L[row] = logf(l);
   }
 }
 
+// The launch overlaps the end of the kernel before it (programmatic dependent launch).
 int launch_combine(const Cache4Args& a, int blocks, int rows, bool f32, cudaStream_t st) {
   KernelTimer kt("cache4_combine", st);
-  const dim3 grid(blocks, std::min(rows, kCombineRows));
-  if (f32) cache4_combine_kernel<float><<<grid, 128, 0, st>>>(a, blocks, rows);
-  else cache4_combine_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(a, blocks, rows);
-  return check_launch("cache4_combine");
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks, rows > 16 ? (rows + 3) / 4 : rows);
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = f32         ? cudaLaunchKernelEx(&cfg, cache4_combine_kernel<float, 4>, a, blocks, rows)
+                        : rows > 16 ? cudaLaunchKernelEx(&cfg, cache4_combine_kernel<__nv_bfloat16, 1>, a, blocks, rows)
+                                    : cudaLaunchKernelEx(&cfg, cache4_combine_kernel<__nv_bfloat16, 4>, a, blocks, rows);
+  if (e != cudaSuccess) return fail(NSA_ERR_LAUNCH, "cache4_combine: %s", cudaGetErrorString(e));
+  return NSA_OK;
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -538,8 +368,7 @@ constexpr int kChunkRows = 128;
 
 static size_t ring_bytes(int dk, int dv) { return (size_t)kC4Warps * kC4Stages * ((dk + dv) / kGroupDims) * kRecBytesPerGroup; }
 
-// thread blocks of a launch: what the device holds at once, or as many as there can be units
-static int grid_blocks(const Cache4Args& a, int rows, int per_sm) {
+int cache4_grid(const Cache4Args& a, int rows, int per_sm) {
   const long long tiles = a.n_sel ? (long long)a.N * ((a.hpg + rows - 1) / rows) : ((long long)a.N * a.hpg + rows - 1) / rows + a.S;
   const long long units = tiles * a.G * (a.n_sel ? a.n_sel : std::max(a.P, 1));
   return (int)std::min<long long>(per_sm * 148, std::max<long long>(units, 1));
@@ -547,14 +376,14 @@ static int grid_blocks(const Cache4Args& a, int rows, int per_sm) {
 
 template <typename T, class Core>
 static size_t core_workspace(const Cache4Args& a) {
-  return split_bytes(grid_blocks(a, Core::kRows, Core::kBlocksPerSm), Core::kRows, a.dv);
+  return split_bytes(cache4_grid(a, Core::kRows, Core::kBlocksPerSm), Core::kRows, a.dv);
 }
 template <typename T, class Core>
 static int launch_core(const Cache4Args& a, const char* name, cudaStream_t st) {
   auto kern = cache4_attn_kernel<T, Core>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kC4Smem);
   if (e != cudaSuccess) return fail(NSA_ERR_LAUNCH, "cache4_attn: cannot reserve shared memory: %s", cudaGetErrorString(e));
-  const int blocks = grid_blocks(a, Core::kRows, Core::kBlocksPerSm);
+  const int blocks = cache4_grid(a, Core::kRows, Core::kBlocksPerSm);
   {
     KernelTimer kt(name, st);
     kern<<<blocks, kC4Threads, ring_bytes(a.dk, a.dv) + Core::extra_smem(a.dk), st>>>(a);
@@ -563,10 +392,7 @@ static int launch_core(const Cache4Args& a, const char* name, cudaStream_t st) {
   return launch_combine(a, blocks, Core::kRows, sizeof(T) == 4, st);
 }
 
-// The tensor-core kernel takes bf16 queries of the head dims that the other tensor-core kernels know; its rows are loaded 16 bytes at a time.
-static bool mma_dims(const Cache4Args& a, int dtype) {
-  return dtype == NSA_BF16 && ((a.dk == 192 && a.dv == 128) || (a.dk == 128 && a.dv == 128) || (a.dk == 64 && a.dv == 64));
-}
+// the tensor-core kernels load their rows 16 bytes at a time
 static bool mma_aligned(const Cache4Args& a) { return (uintptr_t)a.q % 16 == 0 && a.sq_tok % 8 == 0 && a.sq_head % 8 == 0; }
 
 #define NSA_C4_FMA(FN, ...)                                                                              \
@@ -574,11 +400,6 @@ static bool mma_aligned(const Cache4Args& a) { return (uintptr_t)a.q % 16 == 0 &
                                   : FN<float, FmaCore<float, kFmaRows, 4>>(__VA_ARGS__))                 \
                     : (a.dv > 128 ? FN<__nv_bfloat16, FmaCore<__nv_bfloat16, kFmaRows, 8>>(__VA_ARGS__)  \
                                   : FN<__nv_bfloat16, FmaCore<__nv_bfloat16, kFmaRows, 4>>(__VA_ARGS__)))
-#define NSA_C4_MMA(FN, ...)                                                   \
-  (a.dk == 192   ? FN<__nv_bfloat16, MmaCore<6, 4>>(__VA_ARGS__)              \
-   : a.dk == 128 ? FN<__nv_bfloat16, MmaCore<4, 4>>(__VA_ARGS__)              \
-                 : FN<__nv_bfloat16, MmaCore<2, 2>>(__VA_ARGS__))
-
 static int cache4_args(const nsa_cache4_desc* d, Cache4Args& a) {
   NSA_REQUIRE(d, "cache4_attn: null descriptor");
   NSA_REQUIRE(d->N >= 0 && d->S >= 0 && d->P >= 0 && d->n_pages >= 0, "cache4_attn: bad sizes %d/%d/%d/%d", d->N, d->S, d->P, d->n_pages);
@@ -609,9 +430,8 @@ extern "C" NSA_API size_t nsa_cache4_attn_workspace_bytes(const nsa_cache4_desc*
   if (cache4_args(desc, a) != NSA_OK || a.N == 0 || a.S == 0) return 0;
   const int dtype = desc->dtype;
   const size_t fma = NSA_C4_FMA(core_workspace, a);
-  if (!mma_dims(a, dtype)) return fma;
-  const size_t mma = NSA_C4_MMA(core_workspace, a);
-  return std::max({fma, mma, a.n_sel ? 0 : cache4_chunk_workspace(a)});
+  if (dtype != NSA_BF16 || !cache4_mma_dims(a)) return fma;
+  return std::max({fma, cache4_mma_workspace(a), a.n_sel ? 0 : cache4_chunk_workspace(a)});
 }
 
 extern "C" NSA_API int nsa_cache4_attn_fwd(const nsa_cache4_desc* desc, void* workspace, size_t workspace_bytes, void* stream) {
@@ -627,7 +447,7 @@ extern "C" NSA_API int nsa_cache4_attn_fwd(const nsa_cache4_desc* desc, void* wo
   a.ws = (uint8_t*)workspace;
   cudaStream_t st = (cudaStream_t)stream;
   const int dtype = desc->dtype;
-  if (mma_dims(a, dtype) && mma_aligned(a)) {
+  if (dtype == NSA_BF16 && cache4_mma_dims(a) && mma_aligned(a)) {
     // Each request goes to the kernel that suits its rows, by their numbers on the device; a launch that the host can tell to be empty is left out.
     const int most = desc->max_new > 0 ? std::min(desc->max_new, a.N) : a.N;
     const bool chunks = a.n_sel == 0 && (int64_t)most * a.hpg >= kChunkRows;
@@ -638,7 +458,7 @@ extern "C" NSA_API int nsa_cache4_attn_fwd(const nsa_cache4_desc* desc, void* wo
       a.rows_lo = 0;
       a.rows_hi = kChunkRows;
     }
-    return uniform ? NSA_OK : NSA_C4_MMA(launch_core, a, "cache4_attn_mma", st);
+    return uniform ? NSA_OK : launch_mma(a, st);
   }
   return NSA_C4_FMA(launch_core, a, "cache4_attn_fma", st);
 }

@@ -25,11 +25,19 @@ struct Segment {
 
 // what a block leaves about its last segment, if the segment starts there and ends in a later block
 struct SplitRecord {
-  int open, tok0, row0, nrows, g, pad;
-  long long first, last, total;      // the segment's units and the number of all
+  int pieces;                        // blocks that have a part of it, this one the first; 0: there is no such segment
+  int tok0, row0, nrows, g, pad[3];
 };
 
-__device__ __forceinline__ long long share(long long total, int c, int n) { return total * c / n; }
+// Block c of n has units [share(c), share(c + 1)) of total; with fewer units than blocks the first ones have one each.
+__device__ __forceinline__ long long share(long long total, int c, int n) {
+  n = (int)min((long long)n, total);
+  return c >= n ? total : total * c / n;
+}
+__device__ __forceinline__ int block_of(long long total, long long u, int n) {
+  n = (int)min((long long)n, total);
+  return (int)(((u + 1) * n - 1) / total);               // the last c with total * c / n <= u
+}
 
 // KEYS: keys of a unit (one page, or two)
 template <int ROWS, int KEYS = kPageTokens>
@@ -207,6 +215,9 @@ __device__ __forceinline__ float* split_part(const Cache4Args& a, int blocks, in
   return reinterpret_cast<float*>(a.ws + split_rec_bytes(blocks)) + ((size_t)block * 2 + which) * split_part_floats(rows, a.dv);
 }
 
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // row i of a segment: its token and head
 __device__ __forceinline__ int64_t out_row(const Cache4Args& a, const Segment& s, int i) {
   const int f = s.row0 + i;
@@ -217,6 +228,13 @@ __device__ __forceinline__ int64_t out_row(const Cache4Args& a, const Segment& s
 size_t cache4_chunk_workspace(const Cache4Args& a);
 int launch_chunk(const Cache4Args& a, cudaStream_t st);
 
+// bf16 queries on mma.sync (cache4_mma.cu)
+bool cache4_mma_dims(const Cache4Args& a);
+size_t cache4_mma_workspace(const Cache4Args& a);
+int launch_mma(const Cache4Args& a, cudaStream_t st);
+
+// thread blocks of a launch: what the device holds at once, or as many as there can be units
+int cache4_grid(const Cache4Args& a, int rows, int per_sm);
 int launch_combine(const Cache4Args& a, int blocks, int rows, bool f32, cudaStream_t st);
 
 }  // namespace nsa

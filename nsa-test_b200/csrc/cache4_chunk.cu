@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
         if (u < end) {
           w = ChunkPiece{s.tok0, s.row0, s.nrows, s.r, s.g, s.pos0, s.lo + place, (int)min((long long)(s.hi - s.lo - place), end - u), 0, place == 0};
           w.whole = place == 0 && w.n == s.hi - s.lo;
-          if (place == 0 && !w.whole) out = SplitRecord{1, s.tok0, s.row0, s.nrows, s.g, 0, u, u + s.hi - s.lo, walk.total};
+          if (place == 0 && !w.whole) out = SplitRecord{block_of(walk.total, u + s.hi - s.lo - 1, gridDim.x) - (int)blockIdx.x + 1, s.tok0, s.row0, s.nrows, s.g, {}};
         }
         if (lane == 0) {
           bar->piece[c % kChPieces] = w;
@@ -536,6 +536,7 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
   }
 
   // ------------------------------------------------------------ teardown (every thread gets here)
+  pdl_launch();
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && bar->abort) report_timeout(timeouts);
