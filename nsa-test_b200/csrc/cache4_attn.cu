@@ -157,17 +157,25 @@ __global__ void __launch_bounds__(kC4Threads, Core::kBlocksPerSm) cache4_attn_ke
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int groups = (a.dk + a.dv) / kGroupDims, rec_bytes = groups * kRecBytesPerGroup;
   uint8_t* ring = smem + warp * kC4Stages * rec_bytes;
-  uint8_t* extra = smem + kC4Warps * kC4Stages * rec_bytes;
+  uint8_t* extra = smem + max(kC4Warps * kC4Stages * rec_bytes, 4096 * 4);
 
-  Walk<ROWS> walk(a);
-  walk.template start<kC4Threads>(scratch);
+  Walk<ROWS, kPageTokens, 1> walk(a);
+  int* held = reinterpret_cast<int*>(smem);
+  walk.template start<kC4Threads>(scratch, held);
   long long u = share(walk.total, blockIdx.x, gridDim.x);
   const long long end = share(walk.total, blockIdx.x + 1, gridDim.x);
   SplitRecord out{};
-  int place = u < end ? walk.template seek<kC4Threads>(u, scratch) : 0;
+  int place = u < end ? walk.template seek<kC4Threads>(u, scratch, held) : 0;
+  __syncthreads();
   while (u < end) {
     const Segment& s = walk.s;
-    const int p0 = s.lo + place, n = (int)min((long long)(s.hi - p0), end - u);
+    const int p0 = s.lo + place, share_n = (int)min((long long)(walk.length() - place), end - u), n = min(share_n, s.hi - p0);
+    if (n <= 0) {               // no more than what ending the segment counts for
+      u += share_n;
+      place = 0;
+      if (u < end) walk.next();
+      continue;
+    }
     const bool whole = place == 0 && n == s.hi - s.lo;
     const int maxpos = s.pos0 + (s.row0 + s.nrows - 1) / a.hpg;
     const int minlow = a.window > 0 ? s.pos0 + s.row0 / a.hpg - a.window + 1 : 0;
@@ -244,7 +252,7 @@ __global__ void __launch_bounds__(kC4Threads, Core::kBlocksPerSm) cache4_attn_ke
     }
     if (!whole && place == 0)
       out = SplitRecord{block_of(walk.total, u + s.hi - s.lo - 1, gridDim.x) - (int)blockIdx.x + 1, s.tok0, s.row0, s.nrows, s.g, {}};
-    u += n;
+    u += share_n;
     place = 0;
     __syncthreads();
     if (u < end) walk.next();
@@ -366,7 +374,10 @@ constexpr int kC4Smem = 227 * 1024 - 4096;
 // rows (new tokens times heads of a group) from which a request goes to the tensor-memory kernel
 constexpr int kChunkRows = 128;
 
-static size_t ring_bytes(int dk, int dv) { return (size_t)kC4Warps * kC4Stages * ((dk + dv) / kGroupDims) * kRecBytesPerGroup; }
+// records in flight; at first the requests' units are held there
+static size_t ring_bytes(int dk, int dv) {
+  return std::max<size_t>((size_t)kC4Warps * kC4Stages * ((dk + dv) / kGroupDims) * kRecBytesPerGroup, 4096 * 4);
+}
 
 int cache4_grid(const Cache4Args& a, int rows, int per_sm) {
   const long long tiles = a.n_sel ? (long long)a.N * ((a.hpg + rows - 1) / rows) : ((long long)a.N * a.hpg + rows - 1) / rows + a.S;

@@ -39,17 +39,20 @@ __device__ __forceinline__ int block_of(long long total, long long u, int n) {
   return (int)(((u + 1) * n - 1) / total);               // the last c with total * c / n <= u
 }
 
-// KEYS: keys of a unit (one page, or two)
-template <int ROWS, int KEYS = kPageTokens>
+// KEYS: keys of a unit (one page, or two).  OVER: what starting and ending a segment costs, in units, when shares are dealt: they count
+// as units behind the segment's own, and a block whose share of a segment is only of those does nothing for it.
+template <int ROWS, int KEYS, int OVER>
 struct Walk {
+  static constexpr int kChunk = 4096;       // requests whose units are held in shared memory at once
   const Cache4Args& a;
   Segment s;
-  int tile, tiles, len, fresh;       // of the current request
+  int tile, tiles, len, fresh;              // of the current request
   long long total;
 
   __device__ Walk(const Cache4Args& args) : a(args) {}
 
   __device__ __forceinline__ int row_tiles(int n) const { return (n * a.hpg + ROWS - 1) / ROWS; }
+  __device__ __forceinline__ int length() const { return s.hi - s.lo + OVER; }
   // tokens and length of a request: nothing outside [0, N] whatever the arrays hold
   __device__ __forceinline__ void request(int r, int& tok0, int& n, int& length) const {
     const int b = min(max(a.starts[r], 0), a.N), e = min(max(a.starts[r + 1], 0), a.N);
@@ -65,17 +68,6 @@ struct Walk {
     hi = last < 0 ? 0 : min(last / KEYS + 1, (a.P * kPageTokens + KEYS - 1) / KEYS);
     lo = a.window > 0 ? max(first - a.window + 1, 0) / KEYS : 0;
     if (hi <= lo) { lo = 0; hi = 1; }
-  }
-  __device__ __forceinline__ long long units(int r) const {
-    int tok0, n, length;
-    long long sum = 0;
-    request(r, tok0, n, length);
-    for (int t = 0, m = row_tiles(n); t < m; ++t) {
-      int lo, hi;
-      bounds(length, n, t, lo, hi);
-      sum += hi - lo;
-    }
-    return sum * a.G;
   }
 
   __device__ __forceinline__ void set_tile() {
@@ -99,39 +91,77 @@ struct Walk {
     s.pos0 = a.lengths[s.r] - a.starts[s.r + 1] + s.tok0;
   }
 
-  // Number of all units; all threads of the block take part.  Blocks of T threads, scratch of T / 32 + 3 long longs in shared memory.
+  // units (of one group) of requests base .. base + kChunk - 1 into shared memory: a thread per request, or where a request has many
+  // tiles a warp
   template <int T>
-  __device__ __forceinline__ void start(long long* scratch) {
+  __device__ __forceinline__ void fill(int base, int* held) const {
+    const int n = min(kChunk, a.S - base), lane = threadIdx.x & 31;
+    if ((long long)a.N * a.hpg <= 4ll * ROWS * a.S) {
+      for (int i = threadIdx.x; i < n; i += T) {
+        int tok0, fresh, length, sum = 0;
+        request(base + i, tok0, fresh, length);
+        for (int t = 0, m = row_tiles(fresh); t < m; ++t) {
+          int lo, hi;
+          bounds(length, fresh, t, lo, hi);
+          sum += hi - lo + OVER;
+        }
+        held[i] = sum;
+      }
+    } else {
+      for (int i = threadIdx.x >> 5; i < n; i += T / 32) {
+        int tok0, fresh, length, sum = 0;
+        request(base + i, tok0, fresh, length);
+        for (int t = lane, m = row_tiles(fresh); t < m; t += 32) {
+          int lo, hi;
+          bounds(length, fresh, t, lo, hi);
+          sum += hi - lo + OVER;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) held[i] = sum;
+      }
+    }
+    __syncthreads();
+  }
+
+  // Number of all units; all T threads of the block take part.  scratch: T / 32 + 3 long longs of shared memory, held: kChunk ints.
+  template <int T>
+  __device__ __forceinline__ void start(long long* scratch, int* held) {
     if (a.n_sel) {
       const int n = min(max(a.starts[a.S], 0), a.N);
       tiles = (a.hpg + ROWS - 1) / ROWS;
-      total = (long long)n * a.G * tiles * a.n_sel;
       s.lo = 0;
       s.hi = a.n_sel;
+      total = (long long)n * a.G * tiles * length();
       return;
     }
     long long x = 0;
-    for (int r = threadIdx.x; r < a.S; r += T) x += units(r);
+    for (int base = 0; base < a.S; base += kChunk) {
+      if (base) __syncthreads();
+      fill<T>(base, held);
+      for (int i = threadIdx.x; i < min(kChunk, a.S - base); i += T) x += held[i];
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    __syncthreads();
     if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
     __syncthreads();
     total = 0;
     for (int w = 0; w < T / 32; ++w) total += scratch[w];
+    total *= a.G;
     __syncthreads();
   }
   // Segment that unit u (< total) lies in; returns its place within the segment.
   template <int T>
-  __device__ __forceinline__ int seek(long long u, long long* scratch) {
+  __device__ __forceinline__ int seek(long long u, long long* scratch, int* held) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (a.n_sel) {
-      const long long seg = u / a.n_sel;
+      const long long seg = u / length();
       tile = (int)(seg % tiles);
       s.g = (int)(seg / tiles % a.G);
       s.tok0 = (int)(seg / tiles / a.G);
       int lo = 0, up = a.S;                     // last request that starts at or before the token: 32 probes at a time
       while (up - lo > 1) {
-        const int step = (up - lo + 31) / 32, at = lo + (threadIdx.x & 31) * step;
+        const int step = (up - lo + 31) / 32, at = lo + lane * step;
         const unsigned le = __ballot_sync(0xffffffffu, at < up && a.starts[at < up ? at : lo] <= s.tok0);
         const int k = max(31 - __clz(le), 0);
         up = min(up, lo + (k + 1) * step);
@@ -140,45 +170,68 @@ struct Walk {
       s.r = lo;
       set_token();
       set_tile();
-      return (int)(u % a.n_sel);
+      return (int)(u % length());
     }
     long long run = 0;
-    for (int base = 0; base < a.S; base += T) {
-      const int r = base + threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-      const long long x = r < a.S ? units(r) : 0;
-      long long p = x;
+    bool found = false;
+    for (int base = 0; base < a.S && !found; base += kChunk) {
+      if (a.S > kChunk) {
+        __syncthreads();
+        fill<T>(base, held);
+      }
+      for (int i0 = 0; i0 < min(kChunk, a.S - base) && !found; i0 += T) {
+        const int i = i0 + threadIdx.x;
+        const long long x = i < min(kChunk, a.S - base) ? (long long)held[i] * a.G : 0;
+        long long p = x;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, p, o);
-        if (lane >= o) p += y;
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long y = __shfl_up_sync(0xffffffffu, p, o);
+          if (lane >= o) p += y;
+        }
+        __syncthreads();
+        if (lane == 31) scratch[warp] = p;
+        if (threadIdx.x == 0) scratch[T / 32] = -1;
+        __syncthreads();
+        long long before = run;
+        for (int w = 0; w < T / 32; ++w) {
+          if (w < warp) before += scratch[w];
+          run += scratch[w];
+        }
+        p += before;
+        if (u >= p - x && u < p) {
+          scratch[T / 32] = base + i;
+          scratch[T / 32 + 1] = u - (p - x);
+          scratch[T / 32 + 2] = x / a.G;
+        }
+        __syncthreads();
+        found = scratch[T / 32] >= 0;
       }
-      __syncthreads();
-      if (lane == 31) scratch[warp] = p;
-      if (threadIdx.x == 0) scratch[T / 32] = -1;
-      __syncthreads();
-      long long before = run;
-      for (int w = 0; w < T / 32; ++w) {
-        if (w < warp) before += scratch[w];
-        run += scratch[w];
-      }
-      p += before;
-      if (u >= p - x && u < p) {
-        scratch[T / 32] = r;
-        scratch[T / 32 + 1] = u - (p - x);
-      }
-      __syncthreads();
-      if (scratch[T / 32] >= 0) break;
     }
     set_request((int)scratch[T / 32]);
-    long long off = scratch[T / 32 + 1];
+    const long long off = scratch[T / 32 + 1], per = scratch[T / 32 + 2];
     __syncthreads();
-    const long long per = units(s.r) / a.G;
     s.g = (int)(off / per);
     int place = (int)(off % per);
-    for (tile = 0;; ++tile) {
-      set_tile();
-      if (place < s.hi - s.lo || tile + 1 >= tiles) return place;
-      place -= s.hi - s.lo;
+    for (int t0 = 0;; t0 += 32) {               // 32 tiles at a time
+      int lo, hi, p = 0;
+      if (t0 + lane < tiles) {
+        bounds(len, fresh, t0 + lane, lo, hi);
+        p = hi - lo + OVER;
+      }
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, p, o);
+        if (lane >= o) p += y;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, p > place);
+      if (past || t0 + 32 >= tiles) {
+        const int k = past ? __ffs(past) - 1 : tiles - 1 - t0;
+        if (k > 0) place -= __shfl_sync(0xffffffffu, p, k - 1);
+        tile = t0 + k;
+        set_tile();
+        return place;
+      }
+      place -= __shfl_sync(0xffffffffu, p, 31);
     }
   }
   // the segment after this one (there is one)

@@ -28,6 +28,7 @@ using namespace ptx;
 constexpr int kChM = 128, kChN = 128, kChRows = 256, kChThreads = 512;
 constexpr int kChRegsSoftmax = 176, kChRegsUnpack = 104, kChRegsIssue = 56;
 constexpr int kChRegsNeeded = (256 * kChRegsSoftmax + 128 * kChRegsUnpack + 128 * kChRegsIssue + kChThreads - 1) / kChThreads;   // per thread at launch
+constexpr int kChOver = 2;           // see Walk
 constexpr float kChGrow = 8.f;       // log2 units
 
 template <int DK, int DV>
@@ -124,15 +125,16 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
   tc_fence_after();
   const uint32_t tmem = bar->tmem_base;
 
-  Walk<kChRows, kChN> walk(a);
-  walk.template start<kChThreads>(bar->scratch);
+  Walk<kChRows, kChN, kChOver> walk(a);
+  int* held = reinterpret_cast<int*>(smem);       // where queries will be
+  walk.template start<kChThreads>(bar->scratch, held);
   // once any block has given up on a wait the device's results are void: later blocks skip their work
   if (threadIdx.x == 0) bar->scratch[0] = *(volatile const int*)timeouts != 0 ? 0 : walk.total;
   __syncthreads();
   walk.total = bar->scratch[0];
   __syncthreads();
   const long long begin = share(walk.total, blockIdx.x, gridDim.x), end = share(walk.total, blockIdx.x + 1, gridDim.x);
-  const int place0 = begin < end ? walk.template seek<kChThreads>(begin, bar->scratch) : 0;
+  const int place0 = begin < end ? walk.template seek<kChThreads>(begin, bar->scratch, held) : 0;
   __syncthreads();
   // piece number c of the block into registers, its place free again; a wait that runs out reads as the end of the list
   auto take = [&](int c) {
@@ -161,22 +163,25 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
       long long u = begin;
       int place = place0;
       for (int c = 0;; ++c) {
-        if (!mbar_wait_warp(&bar->piece_empty[c % kChPieces], ((c / kChPieces) & 1) ^ 1, abort)) break;
-        const Segment& s = walk.s;
         ChunkPiece w{};
-        if (u < end) {
-          w = ChunkPiece{s.tok0, s.row0, s.nrows, s.r, s.g, s.pos0, s.lo + place, (int)min((long long)(s.hi - s.lo - place), end - u), 0, place == 0};
+        while (u < end && w.n <= 0) {
+          const Segment& s = walk.s;
+          const int share_n = (int)min((long long)(walk.length() - place), end - u);
+          w = ChunkPiece{s.tok0, s.row0, s.nrows, s.r, s.g, s.pos0, s.lo + place, min(share_n, s.hi - s.lo - place), 0, place == 0};
           w.whole = place == 0 && w.n == s.hi - s.lo;
-          if (place == 0 && !w.whole) out = SplitRecord{block_of(walk.total, u + s.hi - s.lo - 1, gridDim.x) - (int)blockIdx.x + 1, s.tok0, s.row0, s.nrows, s.g, {}};
+          if (place == 0 && !w.whole)
+            out = SplitRecord{block_of(walk.total, u + s.hi - s.lo - 1, gridDim.x) - (int)blockIdx.x + 1, s.tok0, s.row0, s.nrows, s.g, {}};
+          u += share_n;
+          place = 0;
+          if (u < end) walk.next();
         }
+        if (w.n < 0) w.n = 0;        // the share ended among what ending a segment counts for
+        if (!mbar_wait_warp(&bar->piece_empty[c % kChPieces], ((c / kChPieces) & 1) ^ 1, abort)) break;
         if (lane == 0) {
           bar->piece[c % kChPieces] = w;
           mbar_arrive(&bar->piece_full[c % kChPieces]);
         }
         if (w.n == 0) break;
-        u += w.n;
-        place = 0;
-        if (u < end) walk.next();
       }
       if (lane == 0) reinterpret_cast<SplitRecord*>(a.ws)[blockIdx.x] = out;
     } else if (warp == 12) {
@@ -251,100 +256,103 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kChRegsUnpack));
     const int wq = warp - 8, n = lane >> 2, j = lane & 3, first = 4 * (n >> 1) + (n & 1);
     const int vg = lane >> 4, vu = (lane >> 2) & 3;
-    bool ok = true;
-    int kc = 0;
-    for (int pc = 0; ok; ++pc) {
-      const ChunkPiece s = take(pc);
-      if (s.n == 0) break;
-      const int maxpos = s.pos0 + (s.row0 + s.nrows - 1) / a.hpg;
-      const int minlow = a.window > 0 ? s.pos0 + s.row0 / a.hpg - a.window + 1 : 0;
-      for (int t = 0; t < s.n; ++t, ++kc) {
-        const int n0 = (s.p0 + t) * kChN;
-        int id0, id1;
-        pages_of(s, s.p0 + t, id0, id1);
-        const int id = wq < 2 ? id0 : id1;         // this warp's two records: half a page
-        const uint8_t* src = a.cache + (((int64_t)max(id, 0) * a.G + s.g) * kRecsPerPage + (wq & 1) * 2) * kRecBytes;
-        // keys: lane (n, j) holds 8 dimensions of tokens n and 8 + n; odd n take the odd group of a pair first, so that the eight
-        // lanes of a store phase fill all eight 16-byte columns
-        uint2 kw[2][GK];
-        __half kscale[2][GK][2];
-        if (id >= 0) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int g = 0; g < GK; ++g) {
-              const int gg = g ^ (n & 1);
-              const uint8_t* rec = src + r * kRecBytes;
-              kw[r][g] = __ldg(reinterpret_cast<const uint2*>(rec + gg * kChunkBytes + lane * 8));
-              const __half* sc = reinterpret_cast<const __half*>(rec + (GK + GV) * kChunkBytes + gg * kChunkScaleBytes) + first;
-              kscale[r][g][0] = __ldg(sc);
-              kscale[r][g][1] = __ldg(sc + 2);
-            }
-        } else {
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int g = 0; g < GK; ++g) {
-              kw[r][g] = make_uint2(0, 0);
-              kscale[r][g][0] = kscale[r][g][1] = __ushort_as_half(0);
-            }
-        }
-        ok = mbar_wait_warp(&bar->k_empty[kc & 1], ((kc >> 1) & 1) ^ 1, abort);
-        if (!ok) break;
-        uint8_t* sK = smem + SM::oK + (kc & 1) * SM::kKBytes;
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int g = 0; g < GK; ++g) {
-            const int gg = g ^ (n & 1), row = (wq * 2 + r) * 16 + n;
-            uint8_t* dst = sK + (g >> 1) * (kChN * 128) + row * 128 + ((((gg & 1) * 4 + j) ^ n) << 4);
-            *reinterpret_cast<uint4*>(dst) = unpack8(kw[r][g].x, __half2half2(kscale[r][g][0]));
-            *reinterpret_cast<uint4*>(dst + 8 * 128) = unpack8(kw[r][g].y, __half2half2(kscale[r][g][1]));
-          }
-        fence_proxy_async();
-        mbar_arrive(&bar->k_full[kc & 1]);
-        // values: lane (group of a pair, dimensions n = 2 u and 2 u + 1, tokens 2 j, 2 j + 1, 8 + 2 j, 8 + 2 j + 1)
-        uint2 v0[2][GV / 2], v1[2][GV / 2], vs[2][GV / 2];
-        if (id >= 0) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int g = 0; g < GV / 2; ++g) {
-              const uint8_t* rec = src + r * kRecBytes;
-              const uint2* c = reinterpret_cast<const uint2*>(rec + (GK + 2 * g + vg) * kChunkBytes);
-              v0[r][g] = __ldg(c + 8 * vu + j);
-              v1[r][g] = __ldg(c + 8 * vu + 4 + j);
-              vs[r][g] = __ldg(reinterpret_cast<const uint2*>(rec + (GK + GV) * kChunkBytes + (GK + 2 * g + vg) * kChunkScaleBytes) + j);
-            }
-        } else {
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int g = 0; g < GV / 2; ++g) v0[r][g] = v1[r][g] = vs[r][g] = make_uint2(0, 0);
-        }
-        // what no row sees may never have been written: nothing of it enters, not as 0 times it either
-        const bool edge = n0 + kChN - 1 > maxpos || n0 < minlow;
-        ok = mbar_wait_warp(&bar->v_empty, (kc & 1) ^ 1, abort);
-        if (!ok) break;
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int g = 0; g < GV / 2; ++g) {
-            uint8_t* dst = smem + SM::oV + g * (kChN * 128);
-            const int rec0 = (wq * 2 + r) * 16;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {             // token 8 (q / 2) + 2 j + q % 2
-              const int row = rec0 + 8 * (q >> 1) + 2 * j + (q & 1);
-              const uint32_t x = q < 2 ? v0[r][g].x : v0[r][g].y, y = q < 2 ? v1[r][g].x : v1[r][g].y, z = q < 2 ? vs[r][g].x : vs[r][g].y;
-              uint32_t sc = __byte_perm(z, z, q & 1 ? 0x3232 : 0x1010);
-              if (edge && (n0 + row > maxpos || n0 + row < minlow)) sc = 0;
-              *reinterpret_cast<uint4*>(dst + row * 128 + (((vg * 4 + vu) ^ (row & 7)) << 4)) =
-                  unpack8(__byte_perm(x, y, q & 1 ? 0x7632 : 0x5410), u2h(sc));
-            }
-          }
-        fence_proxy_async();
-        mbar_arrive(&bar->v_full);
+    // keys: lane (n, j) holds 8 dimensions of tokens n and 8 + n; odd n take the odd group of a pair first, so that the eight lanes of a store
+    // phase fill all eight 16-byte columns.  values: lane (group of a pair, dimensions n = 2 u and 2 u + 1, tokens 2 j, 2 j + 1, 8 + 2 j,
+    // 8 + 2 j + 1).  The loads of a tile are issued while the tile before it is unpacked, those of a piece during the piece before.
+    uint2 kw[2][GK], v0[2][GV / 2], v1[2][GV / 2], vs[2][GV / 2];
+    __half2 kscale[2][GK];
+    ChunkPiece f;                  // piece and tile of the loads
+    int ft = 0, pc = 0, id0 = -1, id1 = -1, id = -1;
+    const uint8_t* src = nullptr;
+    // the tile to load next, and its page: this warp's two records are half of one
+    auto step = [&]() {
+      if (++ft >= f.n) {
+        f = take(pc++);
+        ft = 0;
+        if (f.n == 0) return;
+        pages_of(f, f.p0, id0, id1);
       }
+      id = wq < 2 ? id0 : id1;
+      src = a.cache + (((int64_t)max(id, 0) * a.G + f.g) * kRecsPerPage + (wq & 1) * 2) * kRecBytes;
+      if (ft + 1 < f.n) pages_of(f, f.p0 + ft + 1, id0, id1);
+    };
+    auto load_k = [&]() {
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int g = 0; g < GK; ++g) {
+          const int gg = g ^ (n & 1);
+          const uint8_t* rec = src + r * kRecBytes;
+          kw[r][g] = make_uint2(0, 0);
+          kscale[r][g] = __half2half2(__ushort_as_half(0));
+          if (id >= 0) {
+            kw[r][g] = __ldg(reinterpret_cast<const uint2*>(rec + gg * kChunkBytes + lane * 8));
+            const __half* sc = reinterpret_cast<const __half*>(rec + (GK + GV) * kChunkBytes + gg * kChunkScaleBytes) + first;
+            kscale[r][g] = __halves2half2(__ldg(sc), __ldg(sc + 2));
+          }
+        }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int g = 0; g < GV / 2; ++g) {
+          const uint8_t* rec = src + r * kRecBytes;
+          const uint2* c = reinterpret_cast<const uint2*>(rec + (GK + 2 * g + vg) * kChunkBytes);
+          v0[r][g] = v1[r][g] = vs[r][g] = make_uint2(0, 0);
+          if (id >= 0) {
+            v0[r][g] = __ldg(c + 8 * vu + j);
+            v1[r][g] = __ldg(c + 8 * vu + 4 + j);
+            vs[r][g] = __ldg(reinterpret_cast<const uint2*>(rec + (GK + GV) * kChunkBytes + (GK + 2 * g + vg) * kChunkScaleBytes) + j);
+          }
+        }
+    };
+    f.n = 0;
+    step();
+    if (f.n > 0) {
+      load_k();
+      load_v();
+    }
+    for (int kc = 0; f.n > 0; ++kc) {
+      const int n0 = (f.p0 + ft) * kChN, maxpos = f.pos0 + (f.row0 + f.nrows - 1) / a.hpg;
+      const int minlow = a.window > 0 ? f.pos0 + f.row0 / a.hpg - a.window + 1 : 0;
+      if (!mbar_wait_warp(&bar->k_empty[kc & 1], ((kc >> 1) & 1) ^ 1, abort)) break;
+      uint8_t* sK = smem + SM::oK + (kc & 1) * SM::kKBytes;
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int g = 0; g < GK; ++g) {
+          const int gg = g ^ (n & 1), row = (wq * 2 + r) * 16 + n;
+          uint8_t* dst = sK + (g >> 1) * (kChN * 128) + row * 128 + ((((gg & 1) * 4 + j) ^ n) << 4);
+          *reinterpret_cast<uint4*>(dst) = unpack8(kw[r][g].x, __low2half2(kscale[r][g]));
+          *reinterpret_cast<uint4*>(dst + 8 * 128) = unpack8(kw[r][g].y, __high2half2(kscale[r][g]));
+        }
+      fence_proxy_async();
+      mbar_arrive(&bar->k_full[kc & 1]);
+      step();
+      if (f.n > 0) load_k();
+      // what no row sees may never have been written: nothing of it enters, not as 0 times it either
+      const bool edge = n0 + kChN - 1 > maxpos || n0 < minlow;
+      if (!mbar_wait_warp(&bar->v_empty, (kc & 1) ^ 1, abort)) break;
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int g = 0; g < GV / 2; ++g) {
+          uint8_t* dst = smem + SM::oV + g * (kChN * 128);
+          const int rec0 = (wq * 2 + r) * 16;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {             // token 8 (q / 2) + 2 j + q % 2
+            const int row = rec0 + 8 * (q >> 1) + 2 * j + (q & 1);
+            const uint32_t x = q < 2 ? v0[r][g].x : v0[r][g].y, y = q < 2 ? v1[r][g].x : v1[r][g].y, z = q < 2 ? vs[r][g].x : vs[r][g].y;
+            uint32_t sc = __byte_perm(z, z, q & 1 ? 0x3232 : 0x1010);
+            if (edge && (n0 + row > maxpos || n0 + row < minlow)) sc = 0;
+            *reinterpret_cast<uint4*>(dst + row * 128 + (((vg * 4 + vu) ^ (row & 7)) << 4)) =
+                unpack8(__byte_perm(x, y, q & 1 ? 0x7632 : 0x5410), u2h(sc));
+          }
+        }
+      fence_proxy_async();
+      mbar_arrive(&bar->v_full);
+      if (f.n > 0) load_v();
     }
   } else {
     // ------------------------------------------------------------ softmax and epilogue, one row per thread

@@ -28,6 +28,7 @@ using namespace ptx;
 constexpr int kMmThreads = 128, kMmWarps = 4, kMmRows = 16;
 constexpr int kMmStages = 3;                         // half pages in flight per warp
 constexpr int kMmKeys = 2 * kRecTokens;
+constexpr int kMmOver = 1;                           // see Walk
 constexpr float kMmGrow = 8.f;                       // log2 units
 
 template <int GK, int GV>
@@ -36,6 +37,7 @@ struct MmaSmem {
   static constexpr int oQ = kRingBytes, oC = oQ + GK * 1024, kDynamic = oC + GK * 128;
   static constexpr int kBlocksPerSm = GV > 2 ? 3 : 5;
   static_assert(kMmWarps * kMmRows * GV * 32 * 4 <= kRingBytes, "the warps' results are merged in the ring");
+  static_assert(4096 * 4 <= kRingBytes, "the requests' units are held in the ring");
 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint4& x, uint32_t b0, uint32_t b1, const float4& c) {
@@ -271,8 +273,9 @@ __global__ void __launch_bounds__(kMmThreads, MmaSmem<GK, GV>::kBlocksPerSm) cac
     fence_proxy_async();
   }
 
-  Walk<kMmRows> walk(a);
-  walk.template start<kMmThreads>(scratch);
+  Walk<kMmRows, kPageTokens, kMmOver> walk(a);
+  int* held = reinterpret_cast<int*>(smem);
+  walk.template start<kMmThreads>(scratch, held);
   // once any block has given up on a wait the device's results are void: later blocks skip their work
   if (threadIdx.x == 0) scratch[0] = *(volatile const int*)timeouts != 0 ? 0 : walk.total;
   __syncthreads();
@@ -281,12 +284,20 @@ __global__ void __launch_bounds__(kMmThreads, MmaSmem<GK, GV>::kBlocksPerSm) cac
   long long u = share(walk.total, blockIdx.x, gridDim.x);
   const long long end = share(walk.total, blockIdx.x + 1, gridDim.x);
   SplitRecord out{};
-  int place = u < end ? walk.template seek<kMmThreads>(u, scratch) : 0;
+  int place = u < end ? walk.template seek<kMmThreads>(u, scratch, held) : 0;
+  fence_proxy_async();          // the requests' units were held where copies go
+  __syncthreads();
   int taken = 0;                // half pages this warp has been through: ring place taken % kMmStages, phase of its barrier from the rest
   bool ok = true;
   while (u < end) {
     const Segment& s = walk.s;
-    const int p0 = s.lo + place, n = (int)min((long long)(s.hi - p0), end - u);
+    const int p0 = s.lo + place, share_n = (int)min((long long)(walk.length() - place), end - u), n = min(share_n, s.hi - p0);
+    if (n <= 0) {               // no more than what ending the segment counts for
+      u += share_n;
+      place = 0;
+      if (u < end) walk.next();
+      continue;
+    }
     const bool whole = place == 0 && n == s.hi - s.lo;
     const int minpos = s.pos0 + s.row0 / a.hpg, maxpos = s.pos0 + (s.row0 + s.nrows - 1) / a.hpg;
     const int minlow = a.window > 0 ? minpos - a.window + 1 : 0;
@@ -398,7 +409,7 @@ __global__ void __launch_bounds__(kMmThreads, MmaSmem<GK, GV>::kBlocksPerSm) cac
     }
     if (!whole && place == 0)
       out = SplitRecord{block_of(walk.total, u + s.hi - s.lo - 1, gridDim.x) - (int)blockIdx.x + 1, s.tok0, s.row0, s.nrows, s.g, {}};
-    u += n;
+    u += share_n;
     place = 0;
     fence_proxy_async();        // the results were written where the next copies go
     __syncthreads();
