@@ -26,7 +26,7 @@ namespace nsa {
 using namespace ptx;
 
 constexpr int kChM = 128, kChN = 128, kChRows = 256, kChThreads = 512;
-constexpr int kChRegsSoftmax = 176, kChRegsUnpack = 104, kChRegsIssue = 56;
+constexpr int kChRegsSoftmax = 184, kChRegsUnpack = 88, kChRegsIssue = 56;
 constexpr int kChRegsNeeded = (256 * kChRegsSoftmax + 128 * kChRegsUnpack + 128 * kChRegsIssue + kChThreads - 1) / kChThreads;   // per thread at launch
 constexpr int kChOver = 2;           // see Walk
 constexpr float kChGrow = 8.f;       // log2 units
@@ -34,7 +34,7 @@ constexpr float kChGrow = 8.f;       // log2 units
 template <int DK, int DV>
 struct ChunkSmem {
   static constexpr int kQBytes = kChM * DK * 2, kKBytes = kChN * DK * 2, kVBytes = kChN * DV * 2;
-  static constexpr int oQ = 0, oK = oQ + 2 * kQBytes, oV = oK + 2 * kKBytes, oBar = oV + kVBytes;
+  static constexpr int oQ = 0, oK = oQ + 2 * kQBytes, oV = oK + kKBytes, oBar = oV + 2 * kVBytes;
   static constexpr int kDynamic = oBar + 768 + 1024;       // slack to align the base to the swizzle atom
 };
 
@@ -47,7 +47,7 @@ constexpr int kChPieces = 4, kChRoleWarps = 13;
 struct ChunkBarriers {
   uint64_t piece_full[kChPieces], piece_empty[kChPieces];
   ChunkPiece piece[kChPieces];
-  uint64_t q_full[2], k_full[2], k_empty[2], v_full, v_empty, s_full[2], p_full[2], pv_done[2], o_free[2];
+  uint64_t q_full[2], k_full, k_empty, v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2], o_free[2];
   long long scratch[kChThreads / 32 + 3];
   uint32_t tmem_base;
   int abort;
@@ -102,8 +102,8 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar->q_full[i], 128);
-      mbar_init(&bar->k_full[i], 128);
-      mbar_init(&bar->k_empty[i], 1);
+      mbar_init(&bar->v_full[i], 128);
+      mbar_init(&bar->v_empty[i], 1);
       mbar_init(&bar->s_full[i], 1);
       mbar_init(&bar->p_full[i], 128);
       mbar_init(&bar->pv_done[i], 1);
@@ -113,8 +113,8 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
       mbar_init(&bar->piece_full[i], 1);
       mbar_init(&bar->piece_empty[i], kChRoleWarps);
     }
-    mbar_init(&bar->v_full, 128);
-    mbar_init(&bar->v_empty, 1);
+    mbar_init(&bar->k_full, 128);
+    mbar_init(&bar->k_empty, 1);
     bar->abort = 0;
     fence_barrier_init();
     fence_proxy_async();
@@ -190,12 +190,12 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
       const uint64_t dQ0 = smem_desc_sw128(smem_u32(smem + SM::oQ), 16, 1024);
       const uint64_t dK0 = smem_desc_sw128(smem_u32(smem + SM::oK), 16, 1024);
       const uint64_t dV = smem_desc_sw128(smem_u32(smem + SM::oV), kChN * 128, 1024);
-      auto issue_qk = [&](int i, int ks) {
-        const uint64_t dQ = desc_advance(dQ0, i * SM::kQBytes), dK = desc_advance(dK0, ks * SM::kKBytes);
+      auto issue_qk = [&](int i) {
+        const uint64_t dQ = desc_advance(dQ0, i * SM::kQBytes);
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk)
           umma_ss(tmem + i * 128, desc_advance(dQ, (kk >> 2) * (kChM * 128) + (kk & 3) * 32),
-                  desc_advance(dK, (kk >> 2) * (kChN * 128) + (kk & 3) * 32), idQK, kk > 0);
+                  desc_advance(dK0, (kk >> 2) * (kChN * 128) + (kk & 3) * 32), idQK, kk > 0);
         umma_commit(&bar->s_full[i]);
       };
       bool ok = true;
@@ -206,41 +206,41 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
         const bool two = w.nrows > kChM;
         const int ntile = two ? 2 : 1;
         ok = mbar_wait_warp(&bar->q_full[0], ic0 & 1, abort) && (!two || mbar_wait_warp(&bar->q_full[1], ic1 & 1, abort)) &&
-             mbar_wait_warp(&bar->k_full[kc & 1], (kc >> 1) & 1, abort);
+             mbar_wait_warp(&bar->k_full, kc & 1, abort);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          issue_qk(0, kc & 1);
-          if (two) issue_qk(1, kc & 1);
-          umma_commit(&bar->k_empty[kc & 1]);
+          issue_qk(0);
+          if (two) issue_qk(1);
+          umma_commit(&bar->k_empty);
         }
         __syncwarp();
         for (int j = 0; j < w.n && ok; ++j, ++kc) {
           const bool more = j + 1 < w.n;
-          ok = mbar_wait_warp(&bar->v_full, kc & 1, abort);
+          ok = mbar_wait_warp(&bar->v_full[kc & 1], (kc >> 1) & 1, abort);
           for (int i = 0; i < ntile && ok; ++i) {
             ok = mbar_wait_warp(&bar->p_full[i], (i ? sc1 : sc0) & 1, abort);
             if (ok && j == 0) ok = mbar_wait_warp(&bar->o_free[i], ((i ? ic1 : ic0) & 1) ^ 1, abort);
             if (!ok) break;
-            const int ks = (kc + 1) & 1;
             tc_fence_after();
             if (elect_one()) {
+              const uint64_t dv = desc_advance(dV, (kc & 1) * SM::kVBytes);
 #pragma unroll
               for (int kk = 0; kk < kChN / 16; ++kk)
-                umma_ts(tmem + 256 + i * 128, tmem + i * 128 + kk * 8, desc_advance(dV, kk * 2048), idPV, (j > 0) || (kk > 0));
+                umma_ts(tmem + 256 + i * 128, tmem + i * 128 + kk * 8, desc_advance(dv, kk * 2048), idPV, (j > 0) || (kk > 0));
               umma_commit(&bar->pv_done[i]);
-              if (i + 1 == ntile) umma_commit(&bar->v_empty);
+              if (i + 1 == ntile) umma_commit(&bar->v_empty[kc & 1]);
             }
             __syncwarp();
             if (more) {
               if (i == 0) {
-                ok = mbar_wait_warp(&bar->k_full[ks], ((kc + 1) >> 1) & 1, abort);
+                ok = mbar_wait_warp(&bar->k_full, (kc + 1) & 1, abort);
                 if (!ok) break;
                 tc_fence_after();
               }
               if (elect_one()) {
-                issue_qk(i, ks);
-                if (i + 1 == ntile) umma_commit(&bar->k_empty[ks]);
+                issue_qk(i);
+                if (i + 1 == ntile) umma_commit(&bar->k_empty);
               }
               __syncwarp();
             }
@@ -254,13 +254,13 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
   } else if (warp >= 8) {
     // ------------------------------------------------------------ keys and values: 4 bits in L2 -> fp16 in shared memory
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kChRegsUnpack));
-    const int wq = warp - 8, n = lane >> 2, j = lane & 3, first = 4 * (n >> 1) + (n & 1);
+    const int wq = warp - 8, n = lane >> 2, j = lane & 3;
+    const uint32_t mine = n & 1 ? 0x3232 : 0x1010;       // of a pair of scales, this token's, twice
     const int vg = lane >> 4, vu = (lane >> 2) & 3;
     // keys: lane (n, j) holds 8 dimensions of tokens n and 8 + n; odd n take the odd group of a pair first, so that the eight lanes of a store
     // phase fill all eight 16-byte columns.  values: lane (group of a pair, dimensions n = 2 u and 2 u + 1, tokens 2 j, 2 j + 1, 8 + 2 j,
-    // 8 + 2 j + 1).  The loads of a tile are issued while the tile before it is unpacked, those of a piece during the piece before.
-    uint2 kw[2][GK], v0[2][GV / 2], v1[2][GV / 2], vs[2][GV / 2];
-    __half2 kscale[2][GK];
+    // 8 + 2 j + 1).  A tile's keys are loaded while the tile before it is unpacked; there is time for the rest: keys wait for QK, values have two stages.
+    uint2 kw[2][GK];
     ChunkPiece f;                  // piece and tile of the loads
     int ft = 0, pc = 0, id0 = -1, id1 = -1, id = -1;
     const uint8_t* src = nullptr;
@@ -281,64 +281,64 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
       for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int g = 0; g < GK; ++g) {
-          const int gg = g ^ (n & 1);
-          const uint8_t* rec = src + r * kRecBytes;
           kw[r][g] = make_uint2(0, 0);
-          kscale[r][g] = __half2half2(__ushort_as_half(0));
-          if (id >= 0) {
-            kw[r][g] = __ldg(reinterpret_cast<const uint2*>(rec + gg * kChunkBytes + lane * 8));
-            const __half* sc = reinterpret_cast<const __half*>(rec + (GK + GV) * kChunkBytes + gg * kChunkScaleBytes) + first;
-            kscale[r][g] = __halves2half2(__ldg(sc), __ldg(sc + 2));
-          }
-        }
-    };
-    auto load_v = [&]() {
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int g = 0; g < GV / 2; ++g) {
-          const uint8_t* rec = src + r * kRecBytes;
-          const uint2* c = reinterpret_cast<const uint2*>(rec + (GK + 2 * g + vg) * kChunkBytes);
-          v0[r][g] = v1[r][g] = vs[r][g] = make_uint2(0, 0);
-          if (id >= 0) {
-            v0[r][g] = __ldg(c + 8 * vu + j);
-            v1[r][g] = __ldg(c + 8 * vu + 4 + j);
-            vs[r][g] = __ldg(reinterpret_cast<const uint2*>(rec + (GK + GV) * kChunkBytes + (GK + 2 * g + vg) * kChunkScaleBytes) + j);
-          }
+          if (id >= 0) kw[r][g] = __ldg(reinterpret_cast<const uint2*>(src + r * kRecBytes + (g ^ (n & 1)) * kChunkBytes + lane * 8));
         }
     };
     f.n = 0;
     step();
-    if (f.n > 0) {
-      load_k();
-      load_v();
-    }
+    if (f.n > 0) load_k();
     for (int kc = 0; f.n > 0; ++kc) {
-      const int n0 = (f.p0 + ft) * kChN, maxpos = f.pos0 + (f.row0 + f.nrows - 1) / a.hpg;
+      const int n0 = (f.p0 + ft) * kChN, maxpos = f.pos0 + (f.row0 + f.nrows - 1) / a.hpg, page = id;
       const int minlow = a.window > 0 ? f.pos0 + f.row0 / a.hpg - a.window + 1 : 0;
-      if (!mbar_wait_warp(&bar->k_empty[kc & 1], ((kc >> 1) & 1) ^ 1, abort)) break;
-      uint8_t* sK = smem + SM::oK + (kc & 1) * SM::kKBytes;
+      const uint8_t* rec0 = src;
+      uint2 ks[2][GK];               // four scales: tokens n with its neighbour, and 8 behind them
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int g = 0; g < GK; ++g) {
+          ks[r][g] = make_uint2(0, 0);
+          if (page >= 0)
+            ks[r][g] = __ldg(reinterpret_cast<const uint2*>(rec0 + r * kRecBytes + (GK + GV) * kChunkBytes + (g ^ (n & 1)) * kChunkScaleBytes) + (n >> 1));
+        }
+      if (!mbar_wait_warp(&bar->k_empty, (kc & 1) ^ 1, abort)) break;
+      uint8_t* sK = smem + SM::oK;
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int g = 0; g < GK; ++g) {
           const int gg = g ^ (n & 1), row = (wq * 2 + r) * 16 + n;
           uint8_t* dst = sK + (g >> 1) * (kChN * 128) + row * 128 + ((((gg & 1) * 4 + j) ^ n) << 4);
-          *reinterpret_cast<uint4*>(dst) = unpack8(kw[r][g].x, __low2half2(kscale[r][g]));
-          *reinterpret_cast<uint4*>(dst + 8 * 128) = unpack8(kw[r][g].y, __high2half2(kscale[r][g]));
+          *reinterpret_cast<uint4*>(dst) = unpack8(kw[r][g].x, u2h(__byte_perm(ks[r][g].x, 0, mine)));
+          *reinterpret_cast<uint4*>(dst + 8 * 128) = unpack8(kw[r][g].y, u2h(__byte_perm(ks[r][g].y, 0, mine)));
         }
       fence_proxy_async();
-      mbar_arrive(&bar->k_full[kc & 1]);
+      mbar_arrive(&bar->k_full);
       step();
       if (f.n > 0) load_k();
-      // what no row sees may never have been written: nothing of it enters, not as 0 times it either
-      const bool edge = n0 + kChN - 1 > maxpos || n0 < minlow;
-      if (!mbar_wait_warp(&bar->v_empty, (kc & 1) ^ 1, abort)) break;
+      uint2 v0[2][GV / 2], v1[2][GV / 2], vs[2][GV / 2];
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int g = 0; g < GV / 2; ++g) {
-          uint8_t* dst = smem + SM::oV + g * (kChN * 128);
+          const uint8_t* rec = rec0 + r * kRecBytes;
+          const uint2* c = reinterpret_cast<const uint2*>(rec + (GK + 2 * g + vg) * kChunkBytes);
+          v0[r][g] = v1[r][g] = vs[r][g] = make_uint2(0, 0);
+          if (page >= 0) {
+            v0[r][g] = __ldg(c + 8 * vu + j);
+            v1[r][g] = __ldg(c + 8 * vu + 4 + j);
+            vs[r][g] = __ldg(reinterpret_cast<const uint2*>(rec + (GK + GV) * kChunkBytes + (GK + 2 * g + vg) * kChunkScaleBytes) + j);
+          }
+        }
+      // what no row sees may never have been written: nothing of it enters, not as 0 times it either
+      const bool edge = n0 + kChN - 1 > maxpos || n0 < minlow;
+      if (!mbar_wait_warp(&bar->v_empty[kc & 1], ((kc >> 1) & 1) ^ 1, abort)) break;
+      uint8_t* sV = smem + SM::oV + (kc & 1) * SM::kVBytes;
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int g = 0; g < GV / 2; ++g) {
+          uint8_t* dst = sV + g * (kChN * 128);
           const int rec0 = (wq * 2 + r) * 16;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {             // token 8 (q / 2) + 2 j + q % 2
@@ -351,8 +351,7 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
           }
         }
       fence_proxy_async();
-      mbar_arrive(&bar->v_full);
-      if (f.n > 0) load_v();
+      mbar_arrive(&bar->v_full[kc & 1]);
     }
   } else {
     // ------------------------------------------------------------ softmax and epilogue, one row per thread
@@ -494,27 +493,28 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
       ok = mbar_wait_warp(&bar->pv_done[i], last, abort);
       if (!ok) break;
       tc_fence_after();
-      uint32_t ov[GV][32];
-#pragma unroll
-      for (int c = 0; c < GV; ++c) tmem_ld32(tO + c * 32, ov[c]);
-      tc_wait_ld();
-      tc_fence_before();
-      mbar_arrive(&bar->o_free[i]);
       const int row = i * kChM + r;
-      if (row < s.nrows) {
-        const float rel = l > 0.f ? ex2((m_ref - m_true) * c2) : 1.f;       // results relative to the row's true maximum
-        const float f = s.whole ? (l > 0.f ? 1.f / l : 1.f) : rel;
-        float* part = s.whole ? nullptr : split_part(a, gridDim.x, kChRows, blockIdx.x, s.part);
-        Segment sg;
-        sg.tok0 = s.tok0; sg.row0 = s.row0; sg.g = s.g;
-        const int64_t orow = out_row(a, sg, row);
+      const float rel = l > 0.f ? ex2((m_ref - m_true) * c2) : 1.f;       // results relative to the row's true maximum
+      const float f = s.whole ? (l > 0.f ? 1.f / l : 1.f) : rel;
+      float* part = s.whole ? nullptr : split_part(a, gridDim.x, kChRows, blockIdx.x, s.part);
+      Segment sg;
+      sg.tok0 = s.tok0; sg.row0 = s.row0; sg.g = s.g;
+      const int64_t orow = out_row(a, sg, row);
 #pragma unroll
-        for (int g = 0; g < GV; ++g)
+      for (int g = 0; g < GV; ++g) {
+        uint32_t ov[32];
+        tmem_ld32(tO + g * 32, ov);
+        tc_wait_ld();
+        if (g + 1 == GV) {
+          tc_fence_before();
+          mbar_arrive(&bar->o_free[i]);
+        }
+        if (row < s.nrows) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float x[8];                                                     // dimensions 8 e + 0..7: columns 8 (n / 2) + 2 e + n % 2
+            float x[8];                                                   // dimensions 8 e + 0..7: columns 8 (n / 2) + 2 e + n % 2
 #pragma unroll
-            for (int n = 0; n < 8; ++n) x[n] = __uint_as_float(ov[g][8 * (n >> 1) + 2 * e + (n & 1)]) * f;
+            for (int n = 0; n < 8; ++n) x[n] = __uint_as_float(ov[8 * (n >> 1) + 2 * e + (n & 1)]) * f;
             if (s.whole) {
               uint4 pkt;
               __nv_bfloat162 b[4];
@@ -531,6 +531,9 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
               to[1] = make_float4(x[4], x[5], x[6], x[7]);
             }
           }
+        }
+      }
+      if (row < s.nrows) {
         const float M = m_true == -CUDART_INF_F ? m_true : m_true * row_cl;
         if (s.whole) {
           a.M[orow] = M;
