@@ -51,6 +51,18 @@ struct Walk {
 
   __device__ Walk(const Cache4Args& args) : a(args) {}
 
+  // the walk's place, to lie in shared memory while a kernel needs its registers
+  struct Place {
+    Segment s;
+    int tile, tiles, len, fresh, place;
+    long long u, end, total;
+  };
+  __device__ __forceinline__ void save(Place& p, long long u, long long end, int place) const { p = Place{s, tile, tiles, len, fresh, place, u, end, total}; }
+  __device__ __forceinline__ void restore(const Place& p, long long& u, long long& end, int& place) {
+    s = p.s; tile = p.tile; tiles = p.tiles; len = p.len; fresh = p.fresh; total = p.total;
+    u = p.u; end = p.end; place = p.place;
+  }
+
   __device__ __forceinline__ int row_tiles(int n) const { return (n * a.hpg + ROWS - 1) / ROWS; }
   __device__ __forceinline__ int length() const { return s.hi - s.lo + OVER; }
   // tokens and length of a request: nothing outside [0, N] whatever the arrays hold

@@ -641,58 +641,63 @@ def layer_bwd(desc, q, kv_slc, kv_cmp, kv_win, phi, ctx, dout, shared_kv: bool):
 # paged serving: block tables, the 4-bit cache, attention over it
 # ------------------------------------------------------------------------------------------------
 
-class _on:
-    """``torch.cuda.device`` that costs nothing where the device is the current one already."""
-    __slots__ = ("dev", "ctx")
+_I64X6 = _lib.c_int64 * 6
 
-    def __init__(self, dev):
-        self.dev = dev
 
-    def __enter__(self):
-        self.ctx = None if torch.cuda.current_device() == self.dev.index else torch.cuda.device(self.dev)
-        if self.ctx is not None:
-            self.ctx.__enter__()
+def _same_device(first, *others) -> int:
+    """Index of the CUDA device that all these tensors are on (``require_cuda`` at a tenth of its cost: a decode step makes dozens of
+    such calls of a few microseconds on the GPU)."""
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        require_cuda(first, *others)          # says which
+        raise RuntimeError("NSA kernels run on CUDA tensors only; this package has no CPU path")
+    return index
 
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
+
+def _call(index: int, fn, what: str, *args) -> None:
+    """A library call with ``index`` as the current device and its current stream as the last argument."""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        status = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, stream)
+    if status:
+        check(status, what)
 
 
 def block_tables(cached, new, table, free_pages, tokens: int, page_tokens: int):
     """nsa_block_tables -> (slots [tokens] int64, positions [tokens], starts [S+1], lengths [S], pages [1], int32); table in place."""
-    dev = require_cuda(cached, new, table, free_pages)
+    index = _same_device(table, cached, new, free_pages)
     S, P = table.shape
-    n = 2 * tokens                                    # one allocation: int64 slots first, then the int32 arrays
-    buf = torch.empty(n + tokens + 2 * S + 2, device=dev, dtype=torch.int32)
-    slots = buf[:n].view(torch.int64)
-    positions, starts, lengths, pages = buf[n:].split((tokens, S + 1, S, 1))
+    slots = torch.empty(tokens, device=table.device, dtype=torch.int64)
+    buf = torch.empty(tokens + 2 * S + 2, device=table.device, dtype=torch.int32)
     base = buf.data_ptr()
-    with _on(dev):
-        check(lib.nsa_block_tables(cached.data_ptr(), new.data_ptr(), table.data_ptr(), table.stride(0) if S > 1 else P, free_pages.data_ptr(),
-                                   base, base + 8 * tokens, base + 12 * tokens, base + 12 * tokens + 4 * (S + 1),
-                                   base + 12 * tokens + 4 * (2 * S + 1), S, P, free_pages.numel(), tokens, page_tokens, stream_ptr(dev)),
-              "nsa_block_tables")
-    return slots, positions, starts, lengths, pages
+    _call(index, lib.nsa_block_tables, "nsa_block_tables", cached.data_ptr(), new.data_ptr(), table.data_ptr(), table.stride(0) if S > 1 else P,
+          free_pages.data_ptr(), slots.data_ptr(), base, base + 4 * tokens, base + 4 * (tokens + S + 1), base + 4 * (tokens + 2 * S + 1), S, P,
+          free_pages.shape[0], tokens, page_tokens)
+    return (slots, *buf.split((tokens, S + 1, S, 1)))
 
 
 def cache4_append(k, v, slots, cache) -> None:
     """nsa_cache4_append: k [N,G,dk], v [N,G,dv] of any strides into the slots of cache [pages,G,page bytes]."""
-    dev = require_cuda(k, v, slots, cache)
+    index = _same_device(cache, k, v, slots)
     N, G, dk = k.shape
-    with _on(dev):
-        check(lib.nsa_cache4_append(k.data_ptr(), v.data_ptr(), i64((*k.stride(), *v.stride())), slots.data_ptr(), cache.data_ptr(), N,
-                                    cache.shape[0], G, dk, v.shape[2], dtype_code(k), stream_ptr(dev)), "nsa_cache4_append")
+    _call(index, lib.nsa_cache4_append, "nsa_cache4_append", k.data_ptr(), v.data_ptr(), _I64X6(*k.stride(), *v.stride()), slots.data_ptr(),
+          cache.data_ptr(), N, cache.shape[0], G, dk, v.shape[2], dtype_code(k))
 
 
 def cache4_read(cache, slots, dk: int, dv: int, dtype):
     """nsa_cache4_read -> (k [N,G,dk], v [N,G,dv])."""
-    dev = require_cuda(cache, slots)
-    N, G = slots.numel(), cache.shape[1]
-    k = torch.empty(N, G, dk, device=dev, dtype=dtype)
-    v = torch.empty(N, G, dv, device=dev, dtype=dtype)
-    with _on(dev):
-        check(lib.nsa_cache4_read(cache.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), N, cache.shape[0], G, dk, dv, dtype_code(k),
-                                  stream_ptr(dev)), "nsa_cache4_read")
+    index = _same_device(cache, slots)
+    N, G = slots.shape[0], cache.shape[1]
+    k = torch.empty(N, G, dk, device=cache.device, dtype=dtype)
+    v = torch.empty(N, G, dv, device=cache.device, dtype=dtype)
+    _call(index, lib.nsa_cache4_read, "nsa_cache4_read", cache.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), N, cache.shape[0], G, dk, dv,
+          dtype_code(k))
     return k, v
 
 
@@ -704,18 +709,21 @@ def _cache4_workspace(sizes) -> int:
 
 def cache4_attn(q, cache, table, lengths, starts, indices, dk: int, dv: int, window: int, scale: float, max_new: int, out=None):
     """nsa_cache4_attn_fwd -> (out [N,H,dv], L [N,H], M [N,H]); q [N,H,dk] with unit stride within a head."""
-    dev = require_cuda(q, cache, table, lengths, starts, indices, out)
+    index = _same_device(q, cache, table, lengths, starts, indices, out)
+    dev, dt = q.device, q.dtype
     N, H, _ = q.shape
     S, P = table.shape
+    pages, G, _ = cache.shape
     if out is None:
-        out = torch.empty(N, H, dv, device=dev, dtype=q.dtype)
-    L, M = torch.empty(2, N, H, device=dev, dtype=torch.float32).unbind()
-    sizes = (N, S, P, H, cache.shape[1], dk, dv, cache.shape[0], 0 if indices is None else indices.shape[2], window, max_new, dtype_code(q))
+        out = torch.empty(N, H, dv, device=dev, dtype=dt)
+    L = torch.empty(N, H, device=dev, dtype=torch.float32)
+    M = torch.empty(N, H, device=dev, dtype=torch.float32)
+    sizes = (N, S, P, H, G, dk, dv, pages, 0 if indices is None else indices.shape[2], window, max_new, _lib.BF16 if dt == torch.bfloat16 else _lib.F32)
     nbytes = _cache4_workspace(sizes)
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    desc = _lib.CACHE4_DESC.pack(*sizes, scale, q.stride(0), q.stride(1), table.stride(0) if S > 1 else P, q.data_ptr(), cache.data_ptr(),
-                                 table.data_ptr(), lengths.data_ptr(), starts.data_ptr(), 0 if indices is None else indices.data_ptr(),
-                                 out.data_ptr(), L.data_ptr(), M.data_ptr())
-    with _on(dev):
-        check(lib.nsa_cache4_attn_fwd(desc, ws.data_ptr(), nbytes, stream_ptr(dev)), "nsa_cache4_attn_fwd")
+    sq = q.stride()
+    desc = _lib.CACHE4_DESC.pack(*sizes, scale, sq[0], sq[1], table.stride(0) if S > 1 else P, q.data_ptr(), cache.data_ptr(), table.data_ptr(),
+                                 lengths.data_ptr(), starts.data_ptr(), 0 if indices is None else indices.data_ptr(), out.data_ptr(), L.data_ptr(),
+                                 M.data_ptr())
+    _call(index, lib.nsa_cache4_attn_fwd, "nsa_cache4_attn_fwd", desc, ws.data_ptr(), nbytes)
     return out, L, M
