@@ -106,28 +106,30 @@ __global__ void __launch_bounds__(kTblThreads) block_tables_kernel(const TablesA
 }
 
 // ------------------------------------------------------------------------------------------------ tokens into pages
-// x rounded to the nearest whole number of steps of y, exactly: a quotient that 32 bits round onto k + 1/2 is settled by the sign of
-// x - (k + 1/2) y, which an fma has exact as long as y has few significant bits; true ties go to the even one.
-__device__ __forceinline__ float nearest_multiple(float x, float y) {
-  const float t = __fdiv_rn(x, y), f = floorf(t);
-  if (t - f != 0.5f) return rintf(t);
-  const float d = fmaf(-t, y, x);
-  return d > 0.f ? f + 1.f : d < 0.f ? f : rintf(t);
+// x over step rounded to the nearest whole number, ties to the even one, exactly: the reciprocal's product is off by less than one, and the
+// remainder x - c step is exact (c step has 12 bits at most, the difference no more places than x), so it says whether c is the nearest.
+__device__ __forceinline__ int nearest(float x, float step, float inv, float half) {
+  const float r = fmaf(x, inv, 12582912.f);        // 1.5 * 2^23: the whole number lies in the low bits
+  const float d = fmaf(12582912.f - r, step, x);
+  int c = __float_as_int(r) - 0x4b400000;
+  if (fabsf(d) > half || (fabsf(d) == half && (c & 1))) c += (__float_as_int(d) >> 31) | 1;
+  return c;
 }
 
 // a seventh of `a` to 8 significant bits (multiples of 2^-24 at the low end): what fp16 holds exactly
 __device__ __forceinline__ float scale_of(float a) {
-  const float t = __fdiv_rn(a, 7.f);
-  const int e = max((int)(__float_as_uint(t) >> 23) - 127 - 7, -24);      // (a power of two that t was rounded up to gives the same scale)
-  const float u = __uint_as_float((uint32_t)(e + 127) << 23);
-  return nearest_multiple(a, 7.f * u) * u;                                // 7 u: three bits
+  const float t = a * 0.142857142857f;
+  // (next to a power of two, the one above or below it as the unit gives the same scale)
+  const int e = max((int)(__float_as_uint(t) >> 23) - 127 - 7, -24);
+  const float u = __uint_as_float((uint32_t)(e + 127) << 23), inv_u = __uint_as_float((uint32_t)(127 - e) << 23);
+  return (float)nearest(a, 7.f * u, 0.142857142857f * inv_u, 3.5f * u) * u;
 }
 
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, int64_t stride, bool wide, float (&x)[8]) {
   if (wide) {
     if constexpr (sizeof(T) == 2) {
-      const uint4 w = *reinterpret_cast<const uint4*>(p);
+      const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
       const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -137,7 +139,7 @@ __device__ __forceinline__ void load8(const T* p, int64_t stride, bool wide, flo
     } else {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float4 w = reinterpret_cast<const float4*>(p)[i];
+        const float4 w = __ldg(reinterpret_cast<const float4*>(p) + i);
         x[4 * i] = w.x; x[4 * i + 1] = w.y; x[4 * i + 2] = w.z; x[4 * i + 3] = w.w;
       }
     }
@@ -145,6 +147,55 @@ __device__ __forceinline__ void load8(const T* p, int64_t stride, bool wide, flo
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = Elem<T>::ld(p + i * stride);
   }
+}
+
+// ------------------------------------------------------------------------------------------------
+// A block has 16 tokens of one group.  Tokens of a prompt sit in consecutive slots, and the 16 slots of a record that are all among a
+// call's tokens, one after the other, are dealt with together: the block that has the first of them takes the whole record through shared
+// memory, so that it is read or written in 16-byte pieces.  Other tokens go straight to their bytes.  Four lanes have 32 dimensions of a
+// token, eight each; consecutive lanes have consecutive dimensions.
+// ------------------------------------------------------------------------------------------------
+constexpr int kTokThreads = 256;
+
+struct TokenList {
+  int n, first;                  // how many; index of the record's first token in the call, or -1
+  int token[32];
+  long long slot[32];
+};
+
+__device__ __forceinline__ void build_list(const int64_t* slots, int N, int64_t n_slots, TokenList& list) {
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x, t0 = blockIdx.x * kRecTokens - 15;          // places 0..46: the block's tokens are 15..30
+    const int i0 = t0 + lane, i1 = i0 + 32;
+    const long long s0 = i0 >= 0 && i0 < N ? slots[i0] : -1, s1 = lane < 16 && i1 < N ? slots[i1] : -1;
+    const bool ok0 = s0 >= 0 && s0 < n_slots, ok1 = s1 >= 0 && s1 < n_slots;
+    const long long wrap = __shfl_sync(0xffffffffu, s1, 0);
+    long long up0 = __shfl_down_sync(0xffffffffu, s0, 1), up1 = __shfl_down_sync(0xffffffffu, s1, 1);
+    if (lane == 31) up0 = wrap;
+    const uint64_t follows = (uint64_t)__ballot_sync(0xffffffffu, ok0 && up0 == s0 + 1) | (uint64_t)__ballot_sync(0xffffffffu, ok1 && up1 == s1 + 1) << 32;
+    const uint32_t starts = __ballot_sync(0xffffffffu, ok0 && s0 % kRecTokens == 0 && (follows >> lane & 0x7fffu) == 0x7fffu);   // whole records by their first place
+    const uint32_t mine = starts & 0x7fff8000u;                               // (never two: they are 16 places apart)
+    const int lead = mine ? __ffs(mine) - 1 : -1;
+    // places 15..45 by lane
+    const int place = lane + 15, i = t0 + place;
+    const long long s_hi = __shfl_sync(0xffffffffu, s1, (place - 32) & 31), s_lo = __shfl_sync(0xffffffffu, s0, min(place, 31));
+    const long long slot = place < 32 ? s_lo : s_hi;
+    const bool valid = place < 46 && i < N;
+    const int from = slot >= 0 ? place - (int)(slot % kRecTokens) : -1;
+    const bool covered = valid && slot >= 0 && slot < n_slots && from >= 0 && from < 32 && (starts >> from & 1);
+    const bool take = valid && ((place <= 30 && !covered) || (lead >= 0 && covered && from == lead));
+    const uint32_t who = __ballot_sync(0xffffffffu, take);
+    if (take) {
+      const int at = __popc(who & ((1u << lane) - 1u));
+      list.token[at] = i;
+      list.slot[at] = slot;
+    }
+    if (lane == 0) {
+      list.n = __popc(who);
+      list.first = lead < 0 ? -1 : t0 + lead;
+    }
+  }
+  __syncthreads();
 }
 
 struct StoreArgs {
@@ -157,45 +208,71 @@ struct StoreArgs {
   bool wide_k, wide_v;
 };
 
-// One warp per (token, group), four lanes per 32 dimensions: each holds eight, the largest magnitude goes round the four.  Values
-// are written as 16-bit pieces of four dimensions of one token, so the four lanes first exchange their words.
+// where slot's record of group g begins
+__device__ __forceinline__ int64_t record_at(int64_t slot, int g, int G, int groups) {
+  return (slot / kPageTokens * G + g) * (int64_t)(kRecsPerPage * groups * kRecBytesPerGroup) + (int)(slot & (kPageTokens - 1)) / kRecTokens * (groups * kRecBytesPerGroup);
+}
+
+// codes and scales of chunks c0 .. c1 - 1 of a record
+__device__ __forceinline__ void copy_chunks(uint4* to, const uint4* from, int groups, int c0, int c1) {
+  constexpr int kCodes = kChunkBytes / 16, kScales = kChunkScaleBytes / 16;
+  const int n = (c1 - c0) * kCodes, m = (c1 - c0) * kScales;
+  for (int i = threadIdx.x; i < n + m; i += kTokThreads) {
+    const int at = i < n ? c0 * kCodes + i : groups * kCodes + c0 * kScales + i - n;
+    to[at] = from[at];
+  }
+}
+
 template <typename T>
-__global__ void __launch_bounds__(128) cache4_append_kernel(const StoreArgs a) {
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (item >= (int64_t)a.N * a.G) return;
-  const int tok = (int)(item / a.G), g = (int)(item % a.G), lane = threadIdx.x & 31, j = lane & 3, quad0 = lane & ~3;
-  const int64_t slot = a.slots[tok];
-  if (slot < 0 || slot >= a.n_slots) return;
-  const int groups = a.gk + a.gv, key = (int)(slot % kRecTokens);
-  uint8_t* rec = a.cache + (slot / kPageTokens * a.G + g) * ((int64_t)kRecsPerPage * groups * kRecBytesPerGroup) +
-                 slot % kPageTokens / kRecTokens * (groups * kRecBytesPerGroup);
-  const int t = key >> 3, n = key & 7, pair = n >> 1, odd = n & 1;
-  for (int c0 = 0; c0 < groups; c0 += 8) {
-    const int c = c0 + (lane >> 2);
+__global__ void __launch_bounds__(kTokThreads) cache4_append_kernel(const StoreArgs a) {
+  __shared__ TokenList list;
+  __shared__ __align__(16) uint8_t staged[2 * kMaxHeadDim / kGroupDims * kRecBytesPerGroup];
+  const int g = blockIdx.y, groups = a.gk + a.gv, quad0 = threadIdx.x & 28;
+  const int c0 = blockIdx.z * groups / gridDim.z, c1 = (blockIdx.z + 1) * groups / gridDim.z, cn = c1 - c0;      // this block's chunks
+  const unsigned over = (65536u + cn - 1) / cn;        // idx / cn = idx * over >> 16 for idx (cn - 1) < 65536
+  build_list(a.slots, a.N, a.n_slots, list);
+  const int items = list.n * cn * 4;
+#pragma unroll 2
+  for (int base = 0; base < items; base += kTokThreads) {
+    const int item = base + threadIdx.x, e = (int)((unsigned)(item >> 2) * over >> 16), c = c0 + (item >> 2) - e * cn, j = item & 3;
+    const bool on = item < items;
+    const int tok = on ? list.token[e] : 0;
+    const long long slot = on ? list.slot[e] : -1;
     float x[8] = {};
-    if (c < a.gk)
+    if (on && c < a.gk)
       load8((const T*)a.k + tok * a.sk[0] + g * a.sk[1] + (c * kGroupDims + 8 * j) * a.sk[2], a.sk[2], a.wide_k, x);
-    else if (c < groups)
+    else if (on)
       load8((const T*)a.v + tok * a.sv[0] + g * a.sv[1] + ((c - a.gk) * kGroupDims + 8 * j) * a.sv[2], a.sv[2], a.wide_v, x);
-    float m = 0.f;
+    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -kMaxHeld), kMaxHeld);      // the cache holds finite numbers only
-      m = fmaxf(m, fabsf(x[i]));
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    float m = __uint_as_float(top);
+    if (top > 0x475f2000u) {             // 57120: the cache holds finite numbers only (the four lanes agree)
+      m = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -kMaxHeld), kMaxHeld);
+        m = fmaxf(m, fabsf(x[i]));
+      }
+      m = fmaxf(m, __shfl_xor_sync(0xfu << quad0, m, 1));
+      m = fmaxf(m, __shfl_xor_sync(0xfu << quad0, m, 2));
     }
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const float s = scale_of(m);
+    const float s = scale_of(m), inv = s > 0.f ? __frcp_rn(s) : 0.f, half = s > 0.f ? 0.5f * s : CUDART_INF_F;
     uint32_t w = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float k = s > 0.f ? fminf(fmaxf(nearest_multiple(x[i], s), -7.f), 7.f) : 0.f;
-      w |= (uint32_t)((int)k + 8) << (4 * i);
+      int c8 = nearest(x[i], s, inv, half);
+      if (s < 0x1p-16f) c8 = min(max(c8, -7), 7);      // (a scale of few places may be a good deal below a seventh)
+      w |= (uint32_t)(c8 + 8) << (4 * i);
     }
-    uint32_t we[4];
+    uint32_t we[4];                      // values lie as four dimensions 8 apart: the four lanes exchange their words
 #pragma unroll
-    for (int e = 0; e < 4; ++e) we[e] = __shfl_sync(0xffffffffu, w, quad0 + e);
-    if (c >= groups) continue;
+    for (int i = 0; i < 4; ++i) we[i] = __shfl_sync(0xffffffffu, w, quad0 + i);
+    if (slot < 0 || slot >= a.n_slots) continue;
+    const int key = (int)slot & (kRecTokens - 1), t = key >> 3, n = key & 7, pair = n >> 1, odd = n & 1;
+    uint8_t* rec = list.first >= 0 && tok >= list.first && tok < list.first + kRecTokens ? staged : a.cache + record_at(slot, g, a.G, groups);
     uint8_t* chunk = rec + c * kChunkBytes;
     if (c < a.gk) {
       *reinterpret_cast<uint32_t*>(chunk + (n * 4 + j) * 8 + t * 4) = w;
@@ -205,12 +282,16 @@ __global__ void __launch_bounds__(128) cache4_append_kernel(const StoreArgs a) {
         const int d = 2 * j + b;
         uint32_t h = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) h |= ((we[e] >> (4 * d)) & 15u) << (4 * e);
+        for (int i = 0; i < 4; ++i) h |= ((we[i] >> (4 * d)) & 15u) << (4 * i);
         *reinterpret_cast<uint16_t*>(chunk + (d * 4 + pair) * 8 + (2 * t + odd) * 2) = (uint16_t)h;
       }
     }
     if (j == 0) *reinterpret_cast<__half*>(rec + groups * kChunkBytes + c * kChunkScaleBytes + (4 * pair + 2 * t + odd) * 2) = __float2half_rn(s);
   }
+  if (list.first < 0) return;
+  __syncthreads();
+  uint4* to = reinterpret_cast<uint4*>(a.cache + record_at(a.slots[list.first], g, a.G, groups));
+  copy_chunks(to, reinterpret_cast<const uint4*>(staged), groups, c0, c1);
 }
 
 // ------------------------------------------------------------------------------------------------ and back
@@ -223,21 +304,27 @@ struct LoadArgs {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(128) cache4_read_kernel(const LoadArgs a) {
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (item >= (int64_t)a.N * a.G) return;
-  const int tok = (int)(item / a.G), g = (int)(item % a.G), lane = threadIdx.x & 31, j = lane & 3;
-  const int64_t slot = a.slots[tok];
-  const bool held = slot >= 0 && slot < a.n_slots;
-  const int groups = a.gk + a.gv, key = (int)(held ? slot % kRecTokens : 0);
-  const uint8_t* rec = a.cache + (held ? (slot / kPageTokens * a.G + g) * ((int64_t)kRecsPerPage * groups * kRecBytesPerGroup) +
-                                             slot % kPageTokens / kRecTokens * (groups * kRecBytesPerGroup) : 0);
-  const int t = key >> 3, n = key & 7, pair = n >> 1, odd = n & 1;
-  for (int c = lane >> 2; c < groups; c += 8) {
+__global__ void __launch_bounds__(kTokThreads) cache4_read_kernel(const LoadArgs a) {
+  __shared__ TokenList list;
+  __shared__ __align__(16) uint8_t staged[2 * kMaxHeadDim / kGroupDims * kRecBytesPerGroup];
+  const int g = blockIdx.y, groups = a.gk + a.gv;
+  const int c0 = blockIdx.z * groups / gridDim.z, c1 = (blockIdx.z + 1) * groups / gridDim.z, cn = c1 - c0;
+  const unsigned over = (65536u + cn - 1) / cn;
+  build_list(a.slots, a.N, a.n_slots, list);
+  if (list.first >= 0) {
+    const uint4* from = reinterpret_cast<const uint4*>(a.cache + record_at(a.slots[list.first], g, a.G, groups));
+    copy_chunks(reinterpret_cast<uint4*>(staged), from, groups, c0, c1);
+    __syncthreads();
+  }
+  for (int item = threadIdx.x; item < list.n * cn * 4; item += kTokThreads) {
+    const int e = (int)((unsigned)(item >> 2) * over >> 16), c = c0 + (item >> 2) - e * cn, j = item & 3, tok = list.token[e];
+    const long long slot = list.slot[e];
     alignas(16) T x[8];
     uint32_t w = 0x88888888u;
     float s = 0.f;
-    if (held) {
+    if (slot >= 0 && slot < a.n_slots) {
+      const int key = (int)slot & (kRecTokens - 1), t = key >> 3, n = key & 7, pair = n >> 1, odd = n & 1;
+      const uint8_t* rec = list.first >= 0 && tok >= list.first && tok < list.first + kRecTokens ? staged : a.cache + record_at(slot, g, a.G, groups);
       const uint8_t* chunk = rec + c * kChunkBytes;
       s = __half2float(*reinterpret_cast<const __half*>(rec + groups * kChunkBytes + c * kChunkScaleBytes + (4 * pair + 2 * t + odd) * 2));
       if (c < a.gk) {
@@ -251,15 +338,22 @@ __global__ void __launch_bounds__(128) cache4_read_kernel(const LoadArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) Elem<T>::st(&x[i], (float)((int)((w >> (4 * i)) & 15u) - 8) * s);
-    T* to = c < a.gk ? (T*)a.k + item * (a.gk * kGroupDims) + c * kGroupDims + 8 * j
-                     : (T*)a.v + item * (a.gv * kGroupDims) + (c - a.gk) * kGroupDims + 8 * j;
+    const int64_t row = (int64_t)tok * a.G + g;
+    T* to = c < a.gk ? (T*)a.k + row * (a.gk * kGroupDims) + c * kGroupDims + 8 * j : (T*)a.v + row * (a.gv * kGroupDims) + (c - a.gk) * kGroupDims + 8 * j;
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(x)[i];
   }
 }
 
+// Blocks of 16 tokens; few of them are cut up further by chunks, until there are two for every SM.
+static dim3 token_grid(int N, int G, int groups) {
+  const int64_t blocks = (int64_t)((N + kRecTokens - 1) / kRecTokens) * G;
+  const int cut = (int)((2 * 148 + blocks - 1) / blocks);
+  return dim3((N + kRecTokens - 1) / kRecTokens, G, cut < 1 ? 1 : cut > groups ? groups : cut);
+}
+
 static int check_cache(const char* who, const void* cache, int n_pages, int G, int dk, int dv) {
-  NSA_REQUIRE(n_pages >= 0 && G > 0, "%s: bad page or group count %d/%d", who, n_pages, G);
+  NSA_REQUIRE(n_pages >= 0 && G > 0 && G <= 65535, "%s: bad page or group count %d/%d", who, n_pages, G);
   NSA_REQUIRE(dk > 0 && dv > 0 && dk <= kMaxHeadDim && dv <= kMaxHeadDim && dk % kGroupDims == 0 && dv % kGroupDims == 0,
               "%s: head dims %d/%d are no multiples of %d up to %d", who, dk, dv, kGroupDims, kMaxHeadDim);
   NSA_REQUIRE((uintptr_t)cache % 16 == 0, "%s: the cache must be 16-byte aligned", who);
@@ -309,10 +403,10 @@ extern "C" NSA_API int nsa_cache4_append(const void* k, const void* v, const int
               wide_ok(k, strides6, es), wide_ok(v, strides6 + 3, es)};
   for (int i = 0; i < 3; ++i) { a.sk[i] = strides6[i]; a.sv[i] = strides6[3 + i]; }
   cudaStream_t st = (cudaStream_t)stream;
-  const unsigned grid = (unsigned)(((int64_t)N * G + 3) / 4);
+  const dim3 grid = token_grid(N, G, (dk + dv) / kGroupDims);
   KernelTimer kt("cache4_append", st);
-  if (dtype == NSA_F32) cache4_append_kernel<float><<<grid, 128, 0, st>>>(a);
-  else cache4_append_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(a);
+  if (dtype == NSA_F32) cache4_append_kernel<float><<<grid, kTokThreads, 0, st>>>(a);
+  else cache4_append_kernel<__nv_bfloat16><<<grid, kTokThreads, 0, st>>>(a);
   return check_launch("cache4_append");
 }
 
@@ -326,9 +420,9 @@ extern "C" NSA_API int nsa_cache4_read(const void* cache, const int64_t* slots, 
   NSA_REQUIRE((uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0, "cache4_read: outputs must be 16-byte aligned");
   const LoadArgs a{k, v, slots, (const uint8_t*)cache, (int64_t)n_pages * kPageTokens, N, G, dk / kGroupDims, dv / kGroupDims};
   cudaStream_t st = (cudaStream_t)stream;
-  const unsigned grid = (unsigned)(((int64_t)N * G + 3) / 4);
+  const dim3 grid = token_grid(N, G, (dk + dv) / kGroupDims);
   KernelTimer kt("cache4_read", st);
-  if (dtype == NSA_F32) cache4_read_kernel<float><<<grid, 128, 0, st>>>(a);
-  else cache4_read_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(a);
+  if (dtype == NSA_F32) cache4_read_kernel<float><<<grid, kTokThreads, 0, st>>>(a);
+  else cache4_read_kernel<__nv_bfloat16><<<grid, kTokThreads, 0, st>>>(a);
   return check_launch("cache4_read");
 }
