@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kC4Threads, Core::kBlocksPerSm) cache4_attn_ke
   uint8_t* ring = smem + warp * kC4Stages * rec_bytes;
   uint8_t* extra = smem + max(kC4Warps * kC4Stages * rec_bytes, 4096 * 4);
 
-  Walk<ROWS, kPageTokens, 1> walk(a);
+  Walk<ROWS, kPageTokens, 1, true> walk(a);
   int* held = reinterpret_cast<int*>(smem);
   walk.template start<kC4Threads>(scratch, held);
   long long u = share(walk.total, blockIdx.x, gridDim.x);

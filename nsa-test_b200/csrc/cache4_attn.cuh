@@ -41,7 +41,8 @@ __device__ __forceinline__ int block_of(long long total, long long u, int n) {
 
 // KEYS: keys of a unit (one page, or two).  OVER: what starting and ending a segment costs, in units, when shares are dealt: they count
 // as units behind the segment's own, and a block whose share of a segment is only of those does nothing for it.
-template <int ROWS, int KEYS, int OVER>
+// SEL: the selected form can be asked for.
+template <int ROWS, int KEYS, int OVER, bool SEL>
 struct Walk {
   static constexpr int kChunk = 4096;       // requests whose units are held in shared memory at once
   const Cache4Args& a;
@@ -84,7 +85,7 @@ struct Walk {
 
   __device__ __forceinline__ void set_tile() {
     s.row0 = tile * ROWS;
-    if (a.n_sel) {
+    if (SEL && a.n_sel) {
       s.nrows = min(ROWS, a.hpg - s.row0);
       return;
     }
@@ -139,7 +140,7 @@ struct Walk {
   // Number of all units; all T threads of the block take part.  scratch: T / 32 + 3 long longs of shared memory, held: kChunk ints.
   template <int T>
   __device__ __forceinline__ void start(long long* scratch, int* held) {
-    if (a.n_sel) {
+    if (SEL && a.n_sel) {
       const int n = min(max(a.starts[a.S], 0), a.N);
       tiles = (a.hpg + ROWS - 1) / ROWS;
       s.lo = 0;
@@ -166,7 +167,7 @@ struct Walk {
   template <int T>
   __device__ __forceinline__ int seek(long long u, long long* scratch, int* held) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (a.n_sel) {
+    if (SEL && a.n_sel) {
       const long long seg = u / length();
       tile = (int)(seg % tiles);
       s.g = (int)(seg / tiles % a.G);
@@ -246,13 +247,29 @@ struct Walk {
       place -= __shfl_sync(0xffffffffu, p, 31);
     }
   }
+  // Unit at which block c's share begins.  A boundary inside a segment that is short against a share moves to the segment's nearer end: what
+  // such a segment would cost as two partial results is more than the shares then differ by.  Leaves the walk at that unit, its place in `place`.
+  template <int T>
+  __device__ __forceinline__ long long boundary(int c, int n, long long* scratch, int* held, int& place) {
+    long long u = share(total, c, n);
+    place = 0;
+    if (u >= total) return u;
+    place = seek<T>(u, scratch, held);
+    if (place > 0 && 4ll * length() * n <= total) {
+      const bool up = 2 * place >= length();
+      u += up ? length() - place : -place;
+      place = 0;
+      if (up && u < total) next();
+    }
+    return u;
+  }
   // the segment after this one (there is one)
   __device__ __forceinline__ void next() {
     if (++tile < tiles) return set_tile();
     tile = 0;
     if (++s.g < a.G) return set_tile();
     s.g = 0;
-    if (a.n_sel) {
+    if (SEL && a.n_sel) {
       ++s.tok0;
       set_token();
       return set_tile();

@@ -26,7 +26,7 @@ namespace nsa {
 using namespace ptx;
 
 constexpr int kChM = 128, kChN = 128, kChRows = 256, kChThreads = 512;
-constexpr int kChRegsSoftmax = 184, kChRegsUnpack = 88, kChRegsIssue = 56;
+constexpr int kChRegsSoftmax = 168, kChRegsUnpack = 112, kChRegsIssue = 64;
 constexpr int kChRegsNeeded = (256 * kChRegsSoftmax + 128 * kChRegsUnpack + 128 * kChRegsIssue + kChThreads - 1) / kChThreads;   // per thread at launch
 constexpr int kChOver = 2;           // see Walk
 constexpr float kChGrow = 8.f;       // log2 units
@@ -34,7 +34,7 @@ constexpr float kChGrow = 8.f;       // log2 units
 template <int DK, int DV>
 struct ChunkSmem {
   static constexpr int kQBytes = kChM * DK * 2, kKBytes = kChN * DK * 2, kVBytes = kChN * DV * 2;
-  static constexpr int oQ = 0, oK = oQ + 2 * kQBytes, oV = oK + kKBytes, oBar = oV + 2 * kVBytes;
+  static constexpr int oQ = 0, oK = oQ + 2 * kQBytes, oV = oK + kKBytes, oOut = oV + 2 * kVBytes, oBar = oOut + 8 * 2048;
   static constexpr int kDynamic = oBar + 768 + 1024;       // slack to align the base to the swizzle atom
 };
 
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
   tc_fence_after();
   const uint32_t tmem = bar->tmem_base;
 
-  Walk<kChRows, kChN, kChOver> walk(a);
+  Walk<kChRows, kChN, kChOver, false> walk(a);
   int* held = reinterpret_cast<int*>(smem);       // where queries will be
   walk.template start<kChThreads>(bar->scratch, held);
   // once any block has given up on a wait the device's results are void: later blocks skip their work
@@ -133,8 +133,13 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
   __syncthreads();
   walk.total = bar->scratch[0];
   __syncthreads();
-  const long long begin = share(walk.total, blockIdx.x, gridDim.x), end = share(walk.total, blockIdx.x + 1, gridDim.x);
-  const int place0 = begin < end ? walk.template seek<kChThreads>(begin, bar->scratch, held) : 0;
+  int place0 = 0;
+  long long begin = 0, end = 0;
+#pragma unroll 1
+  for (int c = 1; c >= 0; --c) {          // (one copy of the code: what runs once costs its fetching)
+    end = begin;
+    begin = walk.template boundary<kChThreads>(blockIdx.x + c, gridDim.x, bar->scratch, held, place0);
+  }
   __syncthreads();
   // piece number c of the block into registers, its place free again; a wait that runs out reads as the end of the list
   auto take = [&](int c) {
@@ -360,42 +365,53 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lane_base + i * 128, tO = tmem + lane_base + 256 + i * 128;
     float cl = 0.f;                      // logit of a unit of S
-    int pos = -1;
-    // this thread's row of the current segment into shared memory, as far as the segment has one
-    auto load_q = [&](const ChunkPiece& s) {
-      const int row = i * kChM + r, f = s.row0 + row;
-      const bool there = row < s.nrows;
-      pos = there ? s.pos0 + f / a.hpg : -1;
-      uint4 raw[DK / 8];
-      const uint4* src = reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + (s.tok0 + f / a.hpg) * a.sq_tok + (s.g * a.hpg + f % a.hpg) * a.sq_head);
-      uint32_t mx = 0;
-#pragma unroll
-      for (int c = 0; c < DK / 8; ++c) {
-        raw[c] = there ? src[c] : make_uint4(0, 0, 0, 0);
-        const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx = max(mx, max(w[e] & 0x7fffu, w[e] >> 16 & 0x7fffu));
+    int pos = -1, pos_next = -1;
+    // The rows of a piece into shared memory: copied as they are while the last page of the piece before is worked on (its S has been read, so Q
+    // is free), and turned into fp16 where they lie, a row a thread.  These loops run once a piece: they stay rolled, since what straight
+    // code would save in instructions it loses many times over in fetching them.
+    auto start_q = [&](const ChunkPiece& s) {
+      const int f = s.row0 + i * kChM + r;
+      const bool there = i * kChM + r < s.nrows;
+      pos_next = there ? s.pos0 + f / a.hpg : -1;
+      const int64_t off = there ? (s.tok0 + f / a.hpg) * a.sq_tok + (s.g * a.hpg + f % a.hpg) * a.sq_head : -1;
+#pragma unroll 2
+      for (int it = 0; it < DK / 8; ++it) {
+        const int u = it * 32 + lane, row = u / (DK / 8), c = u % (DK / 8), rr = (warp & 3) * 32 + row;
+        const int64_t at = __shfl_sync(0xffffffffu, off, row);
+        const uint32_t dst = smem_u32(smem + SM::oQ + i * SM::kQBytes + (c >> 3) * (kChM * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"((const __nv_bfloat16*)a.q + max(at, (int64_t)0) + c * 8), "r"(at < 0 ? 0 : 16)
+                     : "memory");
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto finish_q = [&]() {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();
+      uint8_t* mine = smem + SM::oQ + i * SM::kQBytes + r * 128;
+      uint32_t mx = 0;
+#pragma unroll 4
+      for (int c = 0; c < DK / 8; ++c) {
+        const uint4 v = *reinterpret_cast<const uint4*>(mine + (c >> 3) * (kChM * 128) + (((c & 7) ^ (r & 7)) << 4));
+        mx = __vmaxu2(__vmaxu2(mx, v.x & 0x7fff7fffu), __vmaxu2(__vmaxu2(v.y & 0x7fff7fffu, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu));
+      }
+      mx = max(mx & 0xffffu, mx >> 16);
       const int k = mx ? min(14 - ((int)(mx >> 7) - 127), 100) : 0;
       // the scale's sign goes into the row, so that larger S is always the larger logit; scale 0 is a row of zeros
       const float up = __uint_as_float((uint32_t)(k + 127) << 23) * (a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f);
       cl = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * __uint_as_float((uint32_t)(127 - k) << 23);
-      uint8_t* dst = smem + SM::oQ + i * SM::kQBytes + r * 128;
-#pragma unroll
+      pos = pos_next;
+#pragma unroll 2
       for (int c = 0; c < DK / 8; ++c) {
-        const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+        uint4* at = reinterpret_cast<uint4*>(mine + (c >> 3) * (kChM * 128) + (((c & 7) ^ (r & 7)) << 4));
+        const uint4 v = *at;
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
         float x[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           x[2 * e] = __uint_as_float(w[e] << 16) * up;
           x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u) * up;
         }
-        uint4 o;
-        o.x = h2u(__floats2half2_rn(x[0], x[4]));
-        o.y = h2u(__floats2half2_rn(x[1], x[5]));
-        o.z = h2u(__floats2half2_rn(x[2], x[6]));
-        o.w = h2u(__floats2half2_rn(x[3], x[7]));
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * (kChM * 128) + (((c & 7) ^ (r & 7)) << 4)) = o;
+        *at = make_uint4(h2u(__floats2half2_rn(x[0], x[4])), h2u(__floats2half2_rn(x[1], x[5])), h2u(__floats2half2_rn(x[2], x[6])), h2u(__floats2half2_rn(x[3], x[7])));
       }
       fence_proxy_async();
       mbar_arrive(&bar->q_full[i]);
@@ -403,41 +419,68 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
     bool ok = true;
     int sc = 0;                          // key tiles of earlier segments (barrier phases run on)
     int pc = 0;
-    auto take_rows = [&]() {             // the next piece that has rows for this tile
-      ChunkPiece w;
-      do w = take(pc++); while (w.n > 0 && i * kChM >= w.nrows);
-      return w;
+    // Pieces stay in their places while this warp works on them, and are read there: registers are short beside a row's logits.
+    auto release = [&](int c) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar->piece_empty[c % kChPieces]);
     };
-    ChunkPiece s = take_rows();
-    if (s.n > 0) load_q(s);
-    while (s.n > 0) {
+    auto find = [&]() {                  // moves pc on to the next piece that has rows for this tile; false behind the last one
+      for (;; ++pc) {
+        if (!mbar_wait_warp(&bar->piece_full[pc % kChPieces], (pc / kChPieces) & 1, abort)) return false;
+        const ChunkPiece& w = bar->piece[pc % kChPieces];
+        if (w.n == 0 || i * kChM < w.nrows) return w.n > 0;
+        release(pc);
+      }
+    };
+    bool more = find();
+    if (more) {
+      start_q(bar->piece[pc % kChPieces]);
+      finish_q();
+    }
+    while (more) {
+      const int cur = pc;
+      const ChunkPiece& s = bar->piece[cur % kChPieces];
+      const int n = s.n, p0 = s.p0;
       const int row0 = s.row0 + i * kChM, my_pos = pos;
       const float c2 = cl * kLog2e, thr = kChGrow / c2, row_cl = cl;
       const int minpos = s.pos0 + row0 / a.hpg, maxpos = s.pos0 + (s.row0 + min(s.nrows, (i + 1) * kChM) - 1) / a.hpg;
       float m_true = -CUDART_INF_F, m_ref = -CUDART_INF_F, l = 0.f;
       int id0, id1;
-      pages_of(s, s.p0, id0, id1);
-      for (int t = 0; t < s.n && ok; ++t) {
-        const int n0 = (s.p0 + t) * kChN, c0 = id0, c1 = id1;
-        if (t + 1 < s.n) pages_of(s, s.p0 + t + 1, id0, id1);
+      pages_of(s, p0, id0, id1);
+      for (int t = 0; t < n && ok; ++t) {
+        const int n0 = (p0 + t) * kChN, c0 = id0, c1 = id1;
+        if (t + 1 < n) pages_of(s, p0 + t + 1, id0, id1);
         ok = mbar_wait_warp(&bar->s_full[i], (sc + t) & 1, abort);
         if (!ok) break;
         tc_fence_after();
+        if (t + 1 == n) {
+          ++pc;
+          more = find();
+          if (more) start_q(bar->piece[pc % kChPieces]);
+        }
+        if (c0 < 0 || c1 < 0 || n0 + kChN - 1 > minpos || (a.window > 0 && n0 <= maxpos - a.window)) {
+          int clo = a.window > 0 ? my_pos - a.window - n0 : -1, chi = my_pos - n0;       // visible columns: clo < c <= chi
+          if (c0 < 0) clo = max(clo, kPageTokens - 1);
+          if (c1 < 0) chi = min(chi, kPageTokens - 1);
+#pragma unroll 1
+          for (int c = 0; c < kChN; c += 32) {
+            if (__all_sync(0xffffffffu, c > clo && c + 31 <= chi)) continue;
+            uint32_t x[32];
+            tmem_ld32(tS + c, x);
+            tc_wait_ld();
+            // bit e: column c + e is visible
+            const int lo = clo + 1 - c, hi = chi - c;
+            const uint32_t seen = (hi < 0 ? 0u : hi >= 31 ? 0xffffffffu : (2u << hi) - 1u) & (lo <= 0 ? 0xffffffffu : lo > 31 ? 0u : 0xffffffffu << lo);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = seen >> e & 1 ? x[e] : 0xff800000u;
+            tmem_st32(tS + c, x);
+          }
+          tc_wait_st();
+        }
         uint32_t sv[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, sv[c]);
         tc_wait_ld();
-        const bool full = c0 >= 0 && c1 >= 0 && n0 + kChN - 1 <= minpos && (a.window == 0 || n0 > maxpos - a.window);
-        if (!full) {
-          int clo = a.window > 0 ? my_pos - a.window - n0 : -1, chi = my_pos - n0;       // visible columns: clo < c <= chi
-          if (c0 < 0) clo = max(clo, kPageTokens - 1);
-          if (c1 < 0) chi = min(chi, kPageTokens - 1);
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (c * 32 + e <= clo || c * 32 + e > chi) sv[c][e] = 0xff800000u;
-        }
         float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
         for (int c = 0; c < 4; ++c)
@@ -485,11 +528,9 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
         mbar_arrive(&bar->p_full[i]);
       }
       if (!ok) break;
-      const int last = (sc + s.n - 1) & 1;
-      sc += s.n;
-      // the next piece of this tile: its queries go in while the last products run (its S has been read, so Q is free)
-      const ChunkPiece next = take_rows();
-      if (next.n > 0) load_q(next);
+      const int last = (sc + n - 1) & 1;
+      sc += n;
+      if (more) finish_q();
       ok = mbar_wait_warp(&bar->pv_done[i], last, abort);
       if (!ok) break;
       tc_fence_after();
@@ -499,8 +540,10 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
       float* part = s.whole ? nullptr : split_part(a, gridDim.x, kChRows, blockIdx.x, s.part);
       Segment sg;
       sg.tok0 = s.tok0; sg.row0 = s.row0; sg.g = s.g;
-      const int64_t orow = out_row(a, sg, row);
-#pragma unroll
+      const int orow = row < s.nrows ? (int)out_row(a, sg, row) : -1;
+      // 64 bytes of every row of the warp at a time, through shared memory: four lanes a row on their way out instead of one
+      uint8_t* stage = smem + SM::oOut + warp * 2048;
+#pragma unroll 1
       for (int g = 0; g < GV; ++g) {
         uint32_t ov[32];
         tmem_ld32(tO + g * 32, ov);
@@ -509,28 +552,38 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
           tc_fence_before();
           mbar_arrive(&bar->o_free[i]);
         }
-        if (row < s.nrows) {
+        // dimension 8 e + n is column 8 (n / 2) + 2 e + n % 2
+        auto val = [&](int e, int n) { return __uint_as_float(ov[8 * (n >> 1) + 2 * e + (n & 1)]) * f; };
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x[8];                                                   // dimensions 8 e + 0..7: columns 8 (n / 2) + 2 e + n % 2
+        for (int half = 0; half < 2; ++half) {
+          if (s.whole && half) break;
+          uint4* to = reinterpret_cast<uint4*>(stage + lane * 64);
+          if (s.whole) {
 #pragma unroll
-            for (int n = 0; n < 8; ++n) x[n] = __uint_as_float(ov[8 * (n >> 1) + 2 * e + (n & 1)]) * f;
-            if (s.whole) {
-              uint4 pkt;
+            for (int e = 0; e < 4; ++e) {
               __nv_bfloat162 b[4];
 #pragma unroll
-              for (int n = 0; n < 4; ++n) b[n] = __floats2bfloat162_rn(x[2 * n], x[2 * n + 1]);
-              pkt.x = *reinterpret_cast<uint32_t*>(&b[0]);
-              pkt.y = *reinterpret_cast<uint32_t*>(&b[1]);
-              pkt.z = *reinterpret_cast<uint32_t*>(&b[2]);
-              pkt.w = *reinterpret_cast<uint32_t*>(&b[3]);
-              *reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + orow * DV + g * 32 + e * 8) = pkt;
-            } else {
-              float4* to = reinterpret_cast<float4*>(part + row * DV + g * 32 + e * 8);
-              to[0] = make_float4(x[0], x[1], x[2], x[3]);
-              to[1] = make_float4(x[4], x[5], x[6], x[7]);
+              for (int k = 0; k < 4; ++k) b[k] = __floats2bfloat162_rn(val(e, 2 * k), val(e, 2 * k + 1));
+              to[e ^ (lane >> 1 & 3)] = make_uint4(*reinterpret_cast<uint32_t*>(&b[0]), *reinterpret_cast<uint32_t*>(&b[1]),
+                                                   *reinterpret_cast<uint32_t*>(&b[2]), *reinterpret_cast<uint32_t*>(&b[3]));
+            }
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int e = 2 * half + (q >> 1), k = 4 * (q & 1);
+              to[q ^ (lane >> 1 & 3)] = make_uint4(__float_as_uint(val(e, k)), __float_as_uint(val(e, k + 1)), __float_as_uint(val(e, k + 2)), __float_as_uint(val(e, k + 3)));
             }
           }
+          __syncwarp();
+          const int n64 = s.whole ? g : 2 * g + half;
+#pragma unroll
+          for (int it = 0; it < 4; ++it) {
+            const int rr = it * 8 + (lane >> 2), e = lane & 3, at = __shfl_sync(0xffffffffu, orow, rr);
+            const uint4 x = *reinterpret_cast<const uint4*>(stage + rr * 64 + ((e ^ (rr >> 1 & 3)) << 4));
+            uint8_t* base = s.whole ? (uint8_t*)a.out + (int64_t)at * (DV * 2) : (uint8_t*)(part + (row - lane + rr) * DV);
+            if (at >= 0) *reinterpret_cast<uint4*>(base + n64 * 64 + e * 16) = x;
+          }
+          __syncwarp();
         }
       }
       if (row < s.nrows) {
@@ -542,7 +595,7 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
           reinterpret_cast<float2*>(part + kChRows * DV)[row] = make_float2(M, l * rel);
         }
       }
-      s = next;
+      release(cur);
     }
   }
 

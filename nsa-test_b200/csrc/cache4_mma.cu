@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kMmThreads, MmaSmem<GK, GV>::kBlocksPerSm) cac
   // once any block has given up on a wait the device's results are void: later blocks skip their work
   const int gave_up = *(volatile const int*)timeouts;
 
-  using W = Walk<kMmRows, kPageTokens, kMmOver>;
+  using W = Walk<kMmRows, kPageTokens, kMmOver, true>;
   __shared__ typename W::Place at_place;
   {
     W walk(a);
