@@ -371,8 +371,10 @@ int launch_combine(const Cache4Args& a, int blocks, int rows, bool f32, cudaStre
 constexpr int kFmaRows = 8;
 constexpr int kC4Smem = 227 * 1024 - 4096;
 
-// rows (new tokens times heads of a group) from which a request goes to the tensor-memory kernel
-constexpr int kChunkRows = 128;
+// Rows (new tokens times heads of a group) from which a request goes to the tensor-memory kernel: it does 256 rows for the price of one,
+// the mma.sync kernel 16 at a time.  Head dims 192/128, 16 requests of 8000 tokens: 48 rows 69 us against 63, 64 rows 70 against 79, 96 rows
+// 69 against 110; with short caches (a window of 512, 64 rows) 28 against 25, and its fixed cost makes one request of 300 tokens 22 against 14.
+constexpr int kChunkRows = 80;
 
 // records in flight; at first the requests' units are held there
 static size_t ring_bytes(int dk, int dv) {
