@@ -484,6 +484,9 @@ typedef struct nsa_cache4_desc {
   void* out;
   float *L, *M;
 } nsa_cache4_desc;
+/* Sets up the current device's time-out record, which the first attention call on a device does otherwise: that one copies to the device and
+ * cannot be part of a stream capture. */
+NSA_API int nsa_cache4_setup(void);
 NSA_API size_t nsa_cache4_attn_workspace_bytes(const nsa_cache4_desc* desc);
 NSA_API int nsa_cache4_attn_fwd(const nsa_cache4_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
 

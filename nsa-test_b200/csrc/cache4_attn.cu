@@ -3,6 +3,7 @@
 
 #include "attn_args.cuh"
 #include "cache4_attn.cuh"
+#include "fa_sm100.cuh"
 #include "sm100_ptx.cuh"
 
 namespace nsa {
@@ -405,8 +406,8 @@ static int launch_core(const Cache4Args& a, const char* name, cudaStream_t st) {
   return launch_combine(a, blocks, Core::kRows, sizeof(T) == 4, st);
 }
 
-// the tensor-core kernels load their rows 16 bytes at a time
-static bool mma_aligned(const Cache4Args& a) { return (uintptr_t)a.q % 16 == 0 && a.sq_tok % 8 == 0 && a.sq_head % 8 == 0; }
+// the tensor-core kernels load and store their rows 16 bytes at a time
+static bool mma_aligned(const Cache4Args& a) { return (uintptr_t)a.q % 16 == 0 && (uintptr_t)a.out % 16 == 0 && a.sq_tok % 8 == 0 && a.sq_head % 8 == 0; }
 
 #define NSA_C4_FMA(FN, ...)                                                                              \
   (dtype == NSA_F32 ? (a.dv > 128 ? FN<float, FmaCore<float, kFmaRows, 8>>(__VA_ARGS__)                  \
@@ -438,6 +439,11 @@ static int cache4_args(const nsa_cache4_desc* d, Cache4Args& a) {
 
 using namespace nsa;
 
+extern "C" NSA_API int nsa_cache4_setup(void) {
+  if (!fa_timeout_counter()) return fail(NSA_ERR_LAUNCH, "cache4_setup: cannot set up the time-out record of this device");
+  return NSA_OK;
+}
+
 extern "C" NSA_API size_t nsa_cache4_attn_workspace_bytes(const nsa_cache4_desc* desc) {
   Cache4Args a;
   if (cache4_args(desc, a) != NSA_OK || a.N == 0 || a.S == 0) return 0;
@@ -461,17 +467,17 @@ extern "C" NSA_API int nsa_cache4_attn_fwd(const nsa_cache4_desc* desc, void* wo
   cudaStream_t st = (cudaStream_t)stream;
   const int dtype = desc->dtype;
   if (dtype == NSA_BF16 && cache4_mma_dims(a) && mma_aligned(a)) {
-    // Each request goes to the kernel that suits its rows, by their numbers on the device; a launch that the host can tell to be empty is left out.
+    // Each request goes to the kernel that suits its rows, by their numbers on the device.  One launch is enough where no request can have many
+    // rows, or where as many tokens as the requests' bounds allow say that all have: lengths on the device may be less, so the kernel for many
+    // rows then takes every request there is.
     const int most = desc->max_new > 0 ? std::min(desc->max_new, a.N) : a.N;
-    const bool chunks = a.n_sel == 0 && (int64_t)most * a.hpg >= kChunkRows;
-    const bool uniform = desc->max_new > 0 && (int64_t)a.S * desc->max_new == a.N && chunks;
-    if (chunks) {
-      a.rows_lo = kChunkRows;
-      if (int rc = launch_chunk(a, st)) return rc;
-      a.rows_lo = 0;
-      a.rows_hi = kChunkRows;
-    }
-    return uniform ? NSA_OK : launch_mma(a, st);
+    if (a.n_sel || (int64_t)most * a.hpg < kChunkRows) return launch_mma(a, st);
+    if (desc->max_new > 0 && (int64_t)a.S * desc->max_new <= a.N) return launch_chunk(a, st);
+    a.rows_lo = kChunkRows;
+    if (int rc = launch_chunk(a, st)) return rc;
+    a.rows_lo = 0;
+    a.rows_hi = kChunkRows;
+    return launch_mma(a, st);
   }
   return NSA_C4_FMA(launch_core, a, "cache4_attn_fma", st);
 }

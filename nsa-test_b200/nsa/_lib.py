@@ -119,6 +119,7 @@ PROTOTYPES = {
     "nsa_cache4_page_bytes": (c_size_t, [c_int, c_int]),
     "nsa_cache4_append": (c_int, [_P, _P, _I64P, _P, _P] + [c_int] * 6 + [_P]),
     "nsa_cache4_read": (c_int, [_P] * 4 + [c_int] * 6 + [_P]),
+    "nsa_cache4_setup": (c_int, []),
     "nsa_cache4_attn_workspace_bytes": (c_size_t, [_P]),
     "nsa_cache4_attn_fwd": (c_int, [_P, _P, c_size_t, _P]),
 }

@@ -682,6 +682,17 @@ def block_tables(cached, new, table, free_pages, tokens: int, page_tokens: int):
     return (slots, *buf.split((tokens, S + 1, S, 1)))
 
 
+_cache4_ready = set()
+
+
+def cache4_setup(index: int) -> None:
+    """nsa_cache4_setup for device ``index``, once (not while its stream is being captured: the record cannot be set up then)."""
+    if index not in _cache4_ready and not torch.cuda.is_current_stream_capturing():
+        with torch.cuda.device(index):
+            check(lib.nsa_cache4_setup(), "nsa_cache4_setup")
+        _cache4_ready.add(index)
+
+
 def cache4_append(k, v, slots, cache) -> None:
     """nsa_cache4_append: k [N,G,dk], v [N,G,dv] of any strides into the slots of cache [pages,G,page bytes]."""
     index = _same_device(cache, k, v, slots)

@@ -12,6 +12,7 @@ Nothing here waits for the GPU, so a step can be captured into a graph and repla
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple, Optional, Tuple
 
@@ -72,6 +73,14 @@ def block_tables(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, f
     return StepTables(*ops.block_tables(cached, new, table, free_pages, int(tokens), int(page_tokens)))
 
 
+@functools.lru_cache(maxsize=None)
+def _page_bytes(head_dim_qk: int, head_dim_v: int) -> int:
+    nbytes = _lib.lib.nsa_cache4_page_bytes(head_dim_qk, head_dim_v)
+    if nbytes == 0:
+        raise ValueError(f"PagedCache4: head dims {head_dim_qk}/{head_dim_v} are no multiples of 32 up to 256")
+    return nbytes
+
+
 class PagedCache4:
     """Keys and values of ``pages`` pages of 64 tokens in 4 bits with a scale per 32 dimensions.
 
@@ -80,17 +89,16 @@ class PagedCache4:
     """
 
     def __init__(self, storage: torch.Tensor, head_dim_qk: int, head_dim_v: int):
-        nbytes = _lib.lib.nsa_cache4_page_bytes(head_dim_qk, head_dim_v)
-        if nbytes == 0:
-            raise ValueError(f"PagedCache4: head dims {head_dim_qk}/{head_dim_v} are no multiples of 32 up to 256")
+        nbytes = _page_bytes(head_dim_qk, head_dim_v)
         if storage.dtype != torch.uint8 or storage.dim() != 3 or storage.shape[2] != nbytes or not storage.is_contiguous():
             raise ValueError(f"PagedCache4: storage must be contiguous uint8 [pages, groups, {nbytes}], got {storage.dtype} {tuple(storage.shape)}")
         self.storage, self.head_dim_qk, self.head_dim_v = storage, head_dim_qk, head_dim_v
+        if storage.is_cuda:
+            ops.cache4_setup(storage.get_device())
 
     @classmethod
     def empty(cls, pages: int, n_kv_groups: int, head_dim_qk: int, head_dim_v: int, device="cuda") -> "PagedCache4":
-        nbytes = _lib.lib.nsa_cache4_page_bytes(head_dim_qk, head_dim_v)
-        return cls(torch.zeros(pages, n_kv_groups, nbytes, device=device, dtype=torch.uint8), head_dim_qk, head_dim_v)
+        return cls(torch.zeros(pages, n_kv_groups, _page_bytes(head_dim_qk, head_dim_v), device=device, dtype=torch.uint8), head_dim_qk, head_dim_v)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Quantises k ``[N,G,dk]`` and v ``[N,G,dv]`` (any strides) into ``slots [N]``, which are distinct; slots outside the cache (-1)

@@ -431,6 +431,83 @@ def test_same_bits_twice_and_on_another_stream():
         assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(a, b, c))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [HEADS[0], HEADS[2], ODD_HEADS[0]])
+def test_bounds_that_are_not_reached(heads):
+    """As many rows as requests times max_new (a padded step, captured or not), but some requests bring fewer tokens, one none."""
+    s = Served([300, 40, 5, 129], [16, 3, 0, 1], *heads, BF, seed=16)
+    N = s.starts[-1]
+    want = ref.attend(s.q, s.k, s.v, s.lengths, s.starts, s.dk ** -0.5)
+    for rows, most in ((64, 16), (20, 5), (N, 16), (N, 1), (N, 10 ** 6), (N, None)):
+        q = torch.cat((s.q, s.q.new_full((rows - N, *s.q.shape[1:]), math.nan)))
+        o, L, M = s.cache.attend(q, s.table, s.len_dev, s.starts_dev, max_new=most)
+        ref.check((o[:N], L[:N], M[:N]), want, BF, 300, s.dk)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_more_requests_than_are_counted_at_once(dtype):
+    """5000 requests of 1 to 3 cached tokens and 0 to 2 new ones, and one long one behind them all."""
+    rng = random.Random(17)
+    new = [rng.choice([0, 1, 2]) for _ in range(5000)] + [1]
+    s = Served([n + rng.randint(0, 2) for n in new[:-1]] + [700], new, 4, 2, 64, 64, dtype, seed=17, extra=0)
+    s.check()
+    idx = torch.randint(-1, 3, (s.starts[-1], 2, 4), dtype=torch.int32)
+    s.check(indices=idx.cuda())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+def test_scales_that_turn_or_level_the_logits(dtype, new, scale):
+    s = Served([200, 90], [new, 1], *HEADS[2], dtype, seed=18)
+    got = s.cache.attend(s.q, s.table, s.len_dev, s.starts_dev, scale=scale)
+    o, L, M, A, B, V = ref.attend(s.q, s.k, s.v, s.lengths, s.starts, scale)
+    ref.check(got, (o, L, M, A, B.abs(), V), dtype, 200, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 40])
+def test_an_output_tensor_off_its_boundary(new):
+    s = Served([200, 90], [new, 1], *HEADS[0], BF, seed=19)
+    want = ref.attend(s.q, s.k, s.v, s.lengths, s.starts, s.dk ** -0.5)
+    buf = torch.full(((new + 1) * 64 * 128 + 9,), 7.0, device="cuda", dtype=BF)
+    out = buf[3:3 + (new + 1) * 64 * 128].view(new + 1, 64, 128)
+    ref.check(s.cache.attend(s.q, s.table, s.len_dev, s.starts_dev, out=out), want, BF, 200, 192)
+    assert (buf[:3] == 7).all() and (buf[-6:] == 7).all()
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once():
+    a, b = Served([9000, 30], [1, 1], *HEADS[0], BF, seed=20), Served([700, 400], [100, 60], *HEADS[0], BF, seed=21)
+    go = lambda s: s.cache.attend(s.q, s.table, s.len_dev, s.starts_dev)
+    want = go(a), go(b)
+    torch.cuda.synchronize()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    got = [[], []]
+    for _ in range(5):
+        for k, s in enumerate((a, b)):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(go(s))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for k in range(2) for g in got[k] for x, y in zip(g, want[k]))
+
+
+@pytest.mark.gpu
+def test_refuses_after_a_device_time_out():
+    from nsa import _lib as L
+    s = Served([100, 90], [1, 60], *HEADS[2], BF, seed=22)
+    want = s.cache.attend(s.q, s.table, s.len_dev, s.starts_dev)
+    assert L.lib.nsa_selftest_wait_timeout(1 << 16, None) == 0
+    try:
+        with pytest.raises(L.NSAKernelError, match="time-out"):
+            s.cache.attend(s.q, s.table, s.len_dev, s.starts_dev)
+    finally:
+        assert L.lib.nsa_device_timeouts(1) == 1
+    assert all(torch.equal(x, y) for x, y in zip(want, s.cache.attend(s.q, s.table, s.len_dev, s.starts_dev)))
+
+
 # ------------------------------------------------------------------------------------------------ a server's steps
 
 def _serve(steps, H, G, dk, dv, dtype, step_fn):
@@ -478,6 +555,36 @@ def test_a_run_of_steps(heads, dtype):
         return (step, *cache.attend(q, table, step.lengths, step.starts), cache.attend(q, table, step.lengths, step.starts, window=100))
 
     _serve(STEPS, *heads, dtype, step_fn)
+
+
+@pytest.mark.gpu
+def test_a_first_call_under_capture():
+    """A process whose first attention call on the device is captured."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import torch
+from nsa.paged import PagedCache4, block_tables
+i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+c = PagedCache4.empty(4, 2, 64, 64)
+k, q, table = torch.randn(100, 2, 64, device="cuda").bfloat16(), torch.randn(100, 8, 64, device="cuda").bfloat16(), torch.full((1, 3), -1, dtype=torch.int32, device="cuda")
+zero, n, free = i32(0), i32(100), i32(3, 0, 1)
+torch.cuda.synchronize()
+def go():
+    step = block_tables(zero, n, table, free, 100)
+    c.append(k, k, step.slots)
+    return c.attend(q, table, step.lengths, step.starts)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = go()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, go())) and out[0].isfinite().all() and out[0].any()
+"""
+    r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, PYTHONPATH=os.path.join(root, "nsa-test_b200")), capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 @pytest.mark.gpu
