@@ -29,14 +29,19 @@ struct SplitRecord {
   int tok0, row0, nrows, g, pad[3];
 };
 
+// a / b of numbers that are not negative; nearly always both have 32 bits, and dividing those takes a quarter of the instructions
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return ((unsigned long long)(a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
+
 // Block c of n has units [share(c), share(c + 1)) of total; with fewer units than blocks the first ones have one each.
 __device__ __forceinline__ long long share(long long total, int c, int n) {
   n = (int)min((long long)n, total);
-  return c >= n ? total : total * c / n;
+  return c >= n ? total : quotient(total * c, n);
 }
 __device__ __forceinline__ int block_of(long long total, long long u, int n) {
   n = (int)min((long long)n, total);
-  return (int)(((u + 1) * n - 1) / total);               // the last c with total * c / n <= u
+  return (int)quotient((u + 1) * n - 1, total);               // the last c with total * c / n <= u
 }
 
 // KEYS: keys of a unit (one page, or two).  OVER: what starting and ending a segment costs, in units, when shares are dealt: they count
@@ -168,10 +173,10 @@ struct Walk {
   __device__ __forceinline__ int seek(long long u, long long* scratch, int* held) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (SEL && a.n_sel) {
-      const long long seg = u / length();
-      tile = (int)(seg % tiles);
-      s.g = (int)(seg / tiles % a.G);
-      s.tok0 = (int)(seg / tiles / a.G);
+      const long long seg = quotient(u, length()), of_tiles = quotient(seg, tiles), of_groups = quotient(of_tiles, a.G);
+      tile = (int)(seg - of_tiles * tiles);
+      s.g = (int)(of_tiles - of_groups * a.G);
+      s.tok0 = (int)of_groups;
       int lo = 0, up = a.S;                     // last request that starts at or before the token: 32 probes at a time
       while (up - lo > 1) {
         const int step = (up - lo + 31) / 32, at = lo + lane * step;
@@ -183,7 +188,7 @@ struct Walk {
       s.r = lo;
       set_token();
       set_tile();
-      return (int)(u % length());
+      return (int)(u - seg * length());
     }
     long long run = 0;
     bool found = false;
@@ -214,7 +219,7 @@ struct Walk {
         if (u >= p - x && u < p) {
           scratch[T / 32] = base + i;
           scratch[T / 32 + 1] = u - (p - x);
-          scratch[T / 32 + 2] = x / a.G;
+          scratch[T / 32 + 2] = held[i];
         }
         __syncthreads();
         found = scratch[T / 32] >= 0;
@@ -223,8 +228,8 @@ struct Walk {
     set_request((int)scratch[T / 32]);
     const long long off = scratch[T / 32 + 1], per = scratch[T / 32 + 2];
     __syncthreads();
-    s.g = (int)(off / per);
-    int place = (int)(off % per);
+    s.g = (int)quotient(off, per);
+    int place = (int)(off - s.g * per);
     for (int t0 = 0;; t0 += 32) {               // 32 tiles at a time
       int lo, hi, p = 0;
       if (t0 + lane < tiles) {

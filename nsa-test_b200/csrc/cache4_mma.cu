@@ -66,66 +66,68 @@ struct MmaState {
   int pos[2];
 };
 
-// The segment's queries: fragments into shared memory (warp w writes every fourth group), the rows' constants into registers.
+// The segment's queries: fragments into shared memory (warp w forms every fourth group's), the rows' constants into registers.
 template <int GK>
 __device__ __forceinline__ void load_rows(const Cache4Args& a, const Segment& s, uint8_t* sq, float4* sc, MmaState& st) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, j = lane & 3;
-  uint32_t frag[GK][2][4];
-  float sum[GK][2];
+  uint4 raw[2][GK];
+  float up[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int i = n + 8 * h, f = s.row0 + i;
     const bool row = i < s.nrows;
     st.pos[h] = row ? s.pos0 + f / a.hpg : -1;
-    uint4 raw[GK];
     const __nv_bfloat16* src = (const __nv_bfloat16*)a.q + (s.tok0 + f / a.hpg) * a.sq_tok + (s.g * a.hpg + f % a.hpg) * a.sq_head + 8 * j;
+#pragma unroll
+    for (int g = 0; g < GK; ++g) raw[h][g] = row ? *reinterpret_cast<const uint4*>(src + g * kGroupDims) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
     uint32_t mx = 0;
 #pragma unroll
-    for (int g = 0; g < GK; ++g) raw[g] = row ? *reinterpret_cast<const uint4*>(src + g * kGroupDims) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int g = 0; g < GK; ++g) {
-      const uint32_t u[4] = {raw[g].x, raw[g].y, raw[g].z, raw[g].w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mx = max(mx, max(u[e] & 0x7fffu, u[e] >> 16 & 0x7fffu));
-    }
+    for (int g = 0; g < GK; ++g)
+      mx = __vmaxu2(__vmaxu2(mx, raw[h][g].x & 0x7fff7fffu), __vmaxu2(__vmaxu2(raw[h][g].y & 0x7fff7fffu, raw[h][g].z & 0x7fff7fffu), raw[h][g].w & 0x7fff7fffu));
+    mx = max(mx & 0xffffu, mx >> 16);
     mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     const int k = mx ? min(14 - ((int)(mx >> 7) - 127), 100) : 0;
     // the scale's sign goes into the row, so that a larger sum is always the larger logit; scale 0 is a row of zeros
-    const float up = __uint_as_float((uint32_t)(k + 127) << 23) * (a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f);
+    up[h] = __uint_as_float((uint32_t)(k + 127) << 23) * (a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f);
     st.cl[h] = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * __uint_as_float((uint32_t)(127 - k) << 23) * 16777216.f;
     st.c2[h] = st.cl[h] * kLog2e;
-#pragma unroll
-    for (int g = 0; g < GK; ++g) {
-      const uint32_t u[4] = {raw[g].x, raw[g].y, raw[g].z, raw[g].w};
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[2 * e] = __uint_as_float(u[e] << 16) * up;
-        x[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u) * up;
-      }
-      sum[g][h] = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {                                 // dimensions e and e + 4: nibbles e, e + 4
-        const float w = e & 1 ? 0.0625f : 1.f;
-        const __half2 p = __floats2half2_rn(x[e] * w, x[e + 4] * w);
-        sum[g][h] += (__low2float(p) + __high2float(p)) * (e & 1 ? 16.f : 1.f);
-        frag[g][e >> 1][2 * (e & 1) + h] = as_u32(p);
-      }
-      sum[g][h] += __shfl_xor_sync(0xffffffffu, sum[g][h], 1);
-      sum[g][h] += __shfl_xor_sync(0xffffffffu, sum[g][h], 2);
-    }
     st.m[h] = st.lim[h] = st.top[h] = -CUDART_INF_F;
     st.l[h] = 0.f;
   }
 #pragma unroll
   for (int g = 0; g < GK; ++g)
     if ((g & 3) == warp) {
+      uint32_t frag[2][4];
+      float sum[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t u[4] = {raw[h][g].x, raw[h][g].y, raw[h][g].z, raw[h][g].w};
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[2 * e] = __uint_as_float(u[e] << 16) * up[h];
+          x[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u) * up[h];
+        }
+        sum[h] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {                                 // dimensions e and e + 4: nibbles e, e + 4
+          const float w = e & 1 ? 0.0625f : 1.f;
+          const __half2 p = __floats2half2_rn(x[e] * w, x[e + 4] * w);
+          sum[h] += (__low2float(p) + __high2float(p)) * (e & 1 ? 16.f : 1.f);
+          frag[e >> 1][2 * (e & 1) + h] = as_u32(p);
+        }
+        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        *reinterpret_cast<uint4*>(sq + (g * 2 + e) * 512 + lane * 16) = make_uint4(frag[g][e][0], frag[g][e][1], frag[g][e][2], frag[g][e][3]);
-      const float c = -4.76837158203125e-07f;                       // -8 * 2^-24
-      if (j == 0) sc[g * 8 + n] = make_float4(sum[g][0] * c, sum[g][0] * c, sum[g][1] * c, sum[g][1] * c);
+        *reinterpret_cast<uint4*>(sq + (g * 2 + e) * 512 + lane * 16) = make_uint4(frag[e][0], frag[e][1], frag[e][2], frag[e][3]);
+      const float c = -4.76837158203125e-07f;                         // -8 * 2^-24
+      if (j == 0) sc[g * 8 + n] = make_float4(sum[0] * c, sum[0] * c, sum[1] * c, sum[1] * c);
     }
 #pragma unroll
   for (int e = 0; e < 4; ++e)
