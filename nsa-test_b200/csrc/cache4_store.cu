@@ -106,15 +106,17 @@ __global__ void __launch_bounds__(kTblThreads) block_tables_kernel(const TablesA
 }
 
 // ------------------------------------------------------------------------------------------------ tokens into pages
-// x over step rounded to the nearest whole number, ties to the even one, exactly: the reciprocal's product is off by less than one, and the
-// remainder x - c step is exact (c step has 12 bits at most, the difference no more places than x), so it says whether c is the nearest.
-__device__ __forceinline__ int nearest(float x, float step, float inv, float half) {
-  const float r = fmaf(x, inv, 12582912.f);        // 1.5 * 2^23: the whole number lies in the low bits
+// x over step rounded to the nearest whole number c, ties to the even one, exactly, as the bits of 1.5 * 2^23 + c: the reciprocal's product is
+// off by less than one, and the remainder x - c step is exact (c step has 12 bits at most, the difference no more places than x), so it
+// says whether c is the nearest.  (For an odd c a remainder of just a half is too much already: the limit is one place lower.)
+__device__ __forceinline__ int nearest_bits(float x, float step, float inv, float half) {
+  const float r = fmaf(x, inv, 12582912.f);
   const float d = fmaf(12582912.f - r, step, x);
-  int c = __float_as_int(r) - 0x4b400000;
-  if (fabsf(d) > half || (fabsf(d) == half && (c & 1))) c += (__float_as_int(d) >> 31) | 1;
-  return c;
+  int bits = __float_as_int(r);
+  if (fabsf(d) > __int_as_float(__float_as_int(half) - (bits & 1))) bits += (__float_as_int(d) >> 31) | 1;
+  return bits;
 }
+constexpr int kWholeBits = 0x4b400000;               // 1.5 * 2^23
 
 // a seventh of `a` to 8 significant bits (multiples of 2^-24 at the low end): what fp16 holds exactly
 __device__ __forceinline__ float scale_of(float a) {
@@ -122,7 +124,7 @@ __device__ __forceinline__ float scale_of(float a) {
   // (next to a power of two, the one above or below it as the unit gives the same scale)
   const int e = max((int)(__float_as_uint(t) >> 23) - 127 - 7, -24);
   const float u = __uint_as_float((uint32_t)(e + 127) << 23), inv_u = __uint_as_float((uint32_t)(127 - e) << 23);
-  return (float)nearest(a, 7.f * u, 0.142857142857f * inv_u, 3.5f * u) * u;
+  return (float)(nearest_bits(a, 7.f * u, 0.142857142857f * inv_u, 3.5f * u) - kWholeBits) * u;
 }
 
 template <typename T>
@@ -223,26 +225,22 @@ __device__ __forceinline__ void copy_chunks(uint4* to, const uint4* from, int gr
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kTokThreads) cache4_append_kernel(const StoreArgs a) {
-  __shared__ TokenList list;
-  __shared__ __align__(16) uint8_t staged[2 * kMaxHeadDim / kGroupDims * kRecBytesPerGroup];
-  const int g = blockIdx.y, groups = a.gk + a.gv, quad0 = threadIdx.x & 28;
-  const int c0 = blockIdx.z * groups / gridDim.z, c1 = (blockIdx.z + 1) * groups / gridDim.z, cn = c1 - c0;      // this block's chunks
-  const unsigned over = (65536u + cn - 1) / cn;        // idx / cn = idx * over >> 16 for idx (cn - 1) < 65536
-  build_list(a.slots, a.N, a.n_slots, list);
-  const int items = list.n * cn * 4;
+// chunks c0 .. c1 - 1 of the list's tokens, all of the keys or all of the values (V): the lanes of a warp do the same thing
+template <typename T, bool V>
+__device__ __forceinline__ void append_chunks(const StoreArgs& a, const TokenList& list, uint8_t* staged, int g, int c0, int c1) {
+  const int groups = a.gk + a.gv, quad0 = threadIdx.x & 28, cn = c1 - c0, items = list.n * cn * 4;
+  const unsigned over = (65536u + cn - 1) / max(cn, 1);         // idx / cn = idx * over >> 16 for idx (cn - 1) < 65536
+  const T* src = V ? (const T*)a.v + g * a.sv[1] - a.gk * kGroupDims * a.sv[2] : (const T*)a.k + g * a.sk[1];
+  const int64_t s_tok = V ? a.sv[0] : a.sk[0], s_dim = V ? a.sv[2] : a.sk[2];
+  const bool wide = V ? a.wide_v : a.wide_k;
 #pragma unroll 2
   for (int base = 0; base < items; base += kTokThreads) {
-    const int item = base + threadIdx.x, e = (int)((unsigned)(item >> 2) * over >> 16), c = c0 + (item >> 2) - e * cn, j = item & 3;
+    const int item = base + threadIdx.x, idx = item >> 2, e = (int)((unsigned)idx * over >> 16), c = c0 + idx - e * cn, j = item & 3;
     const bool on = item < items;
     const int tok = on ? list.token[e] : 0;
     const long long slot = on ? list.slot[e] : -1;
     float x[8] = {};
-    if (on && c < a.gk)
-      load8((const T*)a.k + tok * a.sk[0] + g * a.sk[1] + (c * kGroupDims + 8 * j) * a.sk[2], a.sk[2], a.wide_k, x);
-    else if (on)
-      load8((const T*)a.v + tok * a.sv[0] + g * a.sv[1] + ((c - a.gk) * kGroupDims + 8 * j) * a.sv[2], a.sv[2], a.wide_v, x);
+    if (on) load8(src + tok * s_tok + (c * kGroupDims + 8 * j) * s_dim, s_dim, wide, x);
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
@@ -260,34 +258,49 @@ __global__ void __launch_bounds__(kTokThreads) cache4_append_kernel(const StoreA
       m = fmaxf(m, __shfl_xor_sync(0xfu << quad0, m, 2));
     }
     const float s = scale_of(m), inv = s > 0.f ? __frcp_rn(s) : 0.f, half = s > 0.f ? 0.5f * s : CUDART_INF_F;
-    uint32_t w = 0;
+    int code[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      int c8 = nearest(x[i], s, inv, half);
-      if (s < 0x1p-16f) c8 = min(max(c8, -7), 7);      // (a scale of few places may be a good deal below a seventh)
-      w |= (uint32_t)(c8 + 8) << (4 * i);
+    for (int i = 0; i < 8; ++i) code[i] = nearest_bits(x[i], s, inv, half);
+    if (__any_sync(0xffffffffu, s < 0x1p-16f)) {         // a scale of few places may be a good deal below a seventh
+#pragma unroll
+      for (int i = 0; i < 8; ++i) code[i] = min(max(code[i], kWholeBits - 7), kWholeBits + 7);
     }
-    uint32_t we[4];                      // values lie as four dimensions 8 apart: the four lanes exchange their words
+    uint32_t w = 0;                                      // sum of (c + 8) 16^i
 #pragma unroll
-    for (int i = 0; i < 4; ++i) we[i] = __shfl_sync(0xffffffffu, w, quad0 + i);
+    for (int i = 7; i >= 0; --i) w = w * 16 + (uint32_t)code[i];
+    w -= (uint32_t)(kWholeBits - 8) * 0x11111111u;
+    uint32_t we[4];                      // values lie as four dimensions 8 apart: the four lanes exchange their words
+    if (V) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) we[i] = __shfl_sync(0xffffffffu, w, quad0 + i) >> (8 * j);
+    }
     if (slot < 0 || slot >= a.n_slots) continue;
     const int key = (int)slot & (kRecTokens - 1), t = key >> 3, n = key & 7, pair = n >> 1, odd = n & 1;
     uint8_t* rec = list.first >= 0 && tok >= list.first && tok < list.first + kRecTokens ? staged : a.cache + record_at(slot, g, a.G, groups);
     uint8_t* chunk = rec + c * kChunkBytes;
-    if (c < a.gk) {
+    if (!V) {
       *reinterpret_cast<uint32_t*>(chunk + (n * 4 + j) * 8 + t * 4) = w;
     } else {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const int d = 2 * j + b;
-        uint32_t h = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h |= ((we[i] >> (4 * d)) & 15u) << (4 * i);
-        *reinterpret_cast<uint16_t*>(chunk + (d * 4 + pair) * 8 + (2 * t + odd) * 2) = (uint16_t)h;
-      }
+      // dimensions n = 2 j and 2 j + 1 of the four lanes, a nibble each
+      const uint32_t lo = (we[0] & 15u) | (we[1] & 15u) << 4 | (we[2] & 15u) << 8 | (we[3] & 15u) << 12;
+      const uint32_t hi = (we[0] >> 4 & 15u) | (we[1] & 0xf0u) | (we[2] & 0xf0u) << 4 | (we[3] & 0xf0u) << 8;
+      uint8_t* to = chunk + (8 * j + pair) * 8 + (2 * t + odd) * 2;
+      *reinterpret_cast<uint16_t*>(to) = (uint16_t)lo;
+      *reinterpret_cast<uint16_t*>(to + 32) = (uint16_t)hi;
     }
     if (j == 0) *reinterpret_cast<__half*>(rec + groups * kChunkBytes + c * kChunkScaleBytes + (4 * pair + 2 * t + odd) * 2) = __float2half_rn(s);
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kTokThreads) cache4_append_kernel(const StoreArgs a) {
+  __shared__ TokenList list;
+  __shared__ __align__(16) uint8_t staged[2 * kMaxHeadDim / kGroupDims * kRecBytesPerGroup];
+  const int g = blockIdx.y, groups = a.gk + a.gv;
+  const int c0 = blockIdx.z * groups / gridDim.z, c1 = (blockIdx.z + 1) * groups / gridDim.z;      // this block's chunks
+  build_list(a.slots, a.N, a.n_slots, list);
+  append_chunks<T, false>(a, list, staged, g, c0, min(c1, a.gk));
+  append_chunks<T, true>(a, list, staged, g, max(c0, a.gk), c1);
   if (list.first < 0) return;
   __syncthreads();
   uint4* to = reinterpret_cast<uint4*>(a.cache + record_at(a.slots[list.first], g, a.G, groups));
@@ -303,21 +316,12 @@ struct LoadArgs {
   int N, G, gk, gv;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kTokThreads) cache4_read_kernel(const LoadArgs a) {
-  __shared__ TokenList list;
-  __shared__ __align__(16) uint8_t staged[2 * kMaxHeadDim / kGroupDims * kRecBytesPerGroup];
-  const int g = blockIdx.y, groups = a.gk + a.gv;
-  const int c0 = blockIdx.z * groups / gridDim.z, c1 = (blockIdx.z + 1) * groups / gridDim.z, cn = c1 - c0;
-  const unsigned over = (65536u + cn - 1) / cn;
-  build_list(a.slots, a.N, a.n_slots, list);
-  if (list.first >= 0) {
-    const uint4* from = reinterpret_cast<const uint4*>(a.cache + record_at(a.slots[list.first], g, a.G, groups));
-    copy_chunks(reinterpret_cast<uint4*>(staged), from, groups, c0, c1);
-    __syncthreads();
-  }
-  for (int item = threadIdx.x; item < list.n * cn * 4; item += kTokThreads) {
-    const int e = (int)((unsigned)(item >> 2) * over >> 16), c = c0 + (item >> 2) - e * cn, j = item & 3, tok = list.token[e];
+template <typename T, bool V>
+__device__ __forceinline__ void read_chunks(const LoadArgs& a, const TokenList& list, const uint8_t* staged, int g, int c0, int c1) {
+  const int groups = a.gk + a.gv, cn = c1 - c0, items = list.n * cn * 4;
+  const unsigned over = (65536u + cn - 1) / max(cn, 1);
+  for (int item = threadIdx.x; item < items; item += kTokThreads) {
+    const int idx = item >> 2, e = (int)((unsigned)idx * over >> 16), c = c0 + idx - e * cn, j = item & 3, tok = list.token[e];
     const long long slot = list.slot[e];
     alignas(16) T x[8];
     uint32_t w = 0x88888888u;
@@ -327,22 +331,39 @@ __global__ void __launch_bounds__(kTokThreads) cache4_read_kernel(const LoadArgs
       const uint8_t* rec = list.first >= 0 && tok >= list.first && tok < list.first + kRecTokens ? staged : a.cache + record_at(slot, g, a.G, groups);
       const uint8_t* chunk = rec + c * kChunkBytes;
       s = __half2float(*reinterpret_cast<const __half*>(rec + groups * kChunkBytes + c * kChunkScaleBytes + (4 * pair + 2 * t + odd) * 2));
-      if (c < a.gk) {
+      if (!V) {
         w = *reinterpret_cast<const uint32_t*>(chunk + (n * 4 + j) * 8 + t * 4);
       } else {
         w = 0;
 #pragma unroll
-        for (int d = 0; d < 8; ++d)
-          w |= (((uint32_t)*reinterpret_cast<const uint16_t*>(chunk + (d * 4 + pair) * 8 + (2 * t + odd) * 2) >> (4 * j)) & 15u) << (4 * d);
+        for (int d = 7; d >= 0; --d)
+          w = w << 4 | (((uint32_t)*reinterpret_cast<const uint16_t*>(chunk + (d * 4 + pair) * 8 + (2 * t + odd) * 2) >> (4 * j)) & 15u);
       }
     }
+    const float s8 = -8.f * s;           // (c - 8) s without a rounding: c s has 12 bits
 #pragma unroll
-    for (int i = 0; i < 8; ++i) Elem<T>::st(&x[i], (float)((int)((w >> (4 * i)) & 15u) - 8) * s);
+    for (int i = 0; i < 8; ++i) Elem<T>::st(&x[i], fmaf((float)((w >> (4 * i)) & 15u), s, s8));
     const int64_t row = (int64_t)tok * a.G + g;
-    T* to = c < a.gk ? (T*)a.k + row * (a.gk * kGroupDims) + c * kGroupDims + 8 * j : (T*)a.v + row * (a.gv * kGroupDims) + (c - a.gk) * kGroupDims + 8 * j;
+    T* to = V ? (T*)a.v + row * (a.gv * kGroupDims) + (c - a.gk) * kGroupDims + 8 * j : (T*)a.k + row * (a.gk * kGroupDims) + c * kGroupDims + 8 * j;
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(x)[i];
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kTokThreads) cache4_read_kernel(const LoadArgs a) {
+  __shared__ TokenList list;
+  __shared__ __align__(16) uint8_t staged[2 * kMaxHeadDim / kGroupDims * kRecBytesPerGroup];
+  const int g = blockIdx.y, groups = a.gk + a.gv;
+  const int c0 = blockIdx.z * groups / gridDim.z, c1 = (blockIdx.z + 1) * groups / gridDim.z;
+  build_list(a.slots, a.N, a.n_slots, list);
+  if (list.first >= 0) {
+    const uint4* from = reinterpret_cast<const uint4*>(a.cache + record_at(a.slots[list.first], g, a.G, groups));
+    copy_chunks(reinterpret_cast<uint4*>(staged), from, groups, c0, c1);
+    __syncthreads();
+  }
+  read_chunks<T, false>(a, list, staged, g, c0, min(c1, a.gk));
+  read_chunks<T, true>(a, list, staged, g, max(c0, a.gk), c1);
 }
 
 // Blocks of 16 tokens; few of them are cut up further by chunks, until there are two for every SM.
