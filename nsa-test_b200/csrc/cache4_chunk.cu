@@ -6,14 +6,17 @@
 //   warps 8-11       unpack a tile's keys and values out of L2 into shared memory: fp16 holds (c - 8) s exactly
 //   warp 13          walks the block's segments and hands the pieces to the others
 //   warp 12          issues the MMAs: S_i = Q_i K^T (both operands in shared memory), O_i += P_i V (P in tensor memory)
-// TMEM columns and the order PV0(j) QK0(j+1) PV1(j) QK1(j+1) are those of the dense forward kernel.  Probabilities are rounded to fp16 (2^-11).
+// TMEM columns and the order PV0(j) QK0(j+1) PV1(j) QK1(j+1) are those of the dense forward kernel.  Probabilities are rounded to fp16 (2^-11);
+// those of the first 64 keys are handed over while the others are formed (head dims 128/128: 1080 -> 1035 us, 192/128: no change).
 //
 // Where a code lies in its word fixes in which order a thread unpacks it for free; the two operands of a product only have to agree.  So
 // eight dimensions of a query and a key lie in the order 0 4 1 5 2 6 3 7, and dimension 8 e + n of a group of 32 values is column
 // 8 (n / 2) + 2 e + n % 2 of the output tile, put back in order when the row is written.
 //
-// Bound by the issue slots of the softmax (a multiply-add, an exponential, a maximum, half a conversion and an addition an element) and the
-// unpacking together, then by the tensor pipe: 2560 clocks a tile of 128 keys at head dims 192/128.
+// Bound by the round trip of a tile: softmax about 2100 clocks (1024 of them the exponentials of 128 keys alone, shared with the other tile's
+// warps), its own two products 1280 at head dims 192/128, handing over on either side of both 400 to 900; about 4400 clocks for two tiles of
+// 128 keys, where the tensor pipe needs 2560.  2048 new tokens behind 30000 earlier ones, 16 query heads a group, 4 groups: 2.2 ms (1150 TFLOP/s)
+// on a chip that is not warm; a long loop of it is slowed by the power limit (2.3 to 2.5 ms).
 #include <algorithm>
 
 #include "attn_args.cuh"
@@ -47,7 +50,7 @@ constexpr int kChPieces = 4, kChRoleWarps = 13;
 struct ChunkBarriers {
   uint64_t piece_full[kChPieces], piece_empty[kChPieces];
   ChunkPiece piece[kChPieces];
-  uint64_t q_full[2], k_full, k_empty, v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2], o_free[2];
+  uint64_t q_full[2], k_full, k_empty, v_full[2], v_empty[2], s_full[2], p_half[2], p_full[2], pv_done[2], o_free[2];
   long long scratch[kChThreads / 32 + 3];
   uint32_t tmem_base;
   int abort;
@@ -77,6 +80,30 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
                "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
+// The issuing warp's instructions, carried out where `on` says so
+__device__ __forceinline__ void mma_ss(uint32_t on, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(on)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t on, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(on)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t on, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(on)
+      : "memory");
+}
 // four codes of each half of a word, nibble by nibble, times the half's scale
 __device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 s) {
   const __half2 bias = __float2half2_rn(-1032.f), sixteenth = __float2half2_rn(0.0625f), bias16 = __float2half2_rn(-72.f);
@@ -105,6 +132,7 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
       mbar_init(&bar->v_full[i], 128);
       mbar_init(&bar->v_empty[i], 1);
       mbar_init(&bar->s_full[i], 1);
+      mbar_init(&bar->p_half[i], 128);
       mbar_init(&bar->p_full[i], 128);
       mbar_init(&bar->pv_done[i], 1);
       mbar_init(&bar->o_free[i], 128);
@@ -191,17 +219,31 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
       if (lane == 0) reinterpret_cast<SplitRecord*>(a.ws)[blockIdx.x] = out;
     } else if (warp == 12) {
       // ---------------------------------------------------------- MMA issuer (warp-uniform loops, one elected lane issues)
+      // One lane issues.  Up to 128 key dimensions the whole warp walks through the instructions, each carried out by its leader, and the code of
+      // either tile is its own: the descriptors of 16 products cost fewer instructions so (head dims 128/128, 2048 tokens behind 30000: 934 us
+      // against 1040 with a branch around them).  With 192 the branch and one copy of the code are faster: 2200 us against 2595.
+      constexpr bool kBranch = DK > 128;
+      constexpr int kCopies = kBranch ? 1 : 2;
       constexpr uint32_t idQK = idesc_f16(kChM, kChN, 0, 0), idPV = idesc_f16(kChM, DV, 0, 1);
       const uint64_t dQ0 = smem_desc_sw128(smem_u32(smem + SM::oQ), 16, 1024);
       const uint64_t dK0 = smem_desc_sw128(smem_u32(smem + SM::oK), 16, 1024);
       const uint64_t dV = smem_desc_sw128(smem_u32(smem + SM::oV), kChN * 128, 1024);
-      auto issue_qk = [&](int i) {
+      const uint32_t leader = elect_one();
+      auto by_leader = [&](auto&& f) {
+        if constexpr (kBranch) {
+          if (leader) f(1u);
+          __syncwarp();
+        } else {
+          f(leader);
+        }
+      };
+      auto issue_qk = [&](uint32_t on, int i) {
         const uint64_t dQ = desc_advance(dQ0, i * SM::kQBytes);
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk)
-          umma_ss(tmem + i * 128, desc_advance(dQ, (kk >> 2) * (kChM * 128) + (kk & 3) * 32),
-                  desc_advance(dK0, (kk >> 2) * (kChN * 128) + (kk & 3) * 32), idQK, kk > 0);
-        umma_commit(&bar->s_full[i]);
+          mma_ss(on, tmem + i * 128, desc_advance(dQ, (kk >> 2) * (kChM * 128) + (kk & 3) * 32),
+                 desc_advance(dK0, (kk >> 2) * (kChN * 128) + (kk & 3) * 32), idQK, kk > 0);
+        commit(on, &bar->s_full[i]);
       };
       bool ok = true;
       int kc = 0, ic0 = 0, ic1 = 0, sc0 = 0, sc1 = 0;     // key tiles; segments and key tiles of either MMA tile so far
@@ -214,40 +256,46 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
              mbar_wait_warp(&bar->k_full, kc & 1, abort);
         if (!ok) break;
         tc_fence_after();
-        if (elect_one()) {
-          issue_qk(0);
-          if (two) issue_qk(1);
-          umma_commit(&bar->k_empty);
-        }
-        __syncwarp();
+        by_leader([&](uint32_t on) {
+          issue_qk(on, 0);
+          if (two) issue_qk(on, 1);
+          commit(on, &bar->k_empty);
+        });
         for (int j = 0; j < w.n && ok; ++j, ++kc) {
           const bool more = j + 1 < w.n;
           ok = mbar_wait_warp(&bar->v_full[kc & 1], (kc >> 1) & 1, abort);
-          for (int i = 0; i < ntile && ok; ++i) {
-            ok = mbar_wait_warp(&bar->p_full[i], (i ? sc1 : sc0) & 1, abort);
+#pragma unroll kCopies
+          for (int i = 0; i < 2; ++i) {
+            if (i >= ntile || !ok) break;
+            ok = mbar_wait_warp(&bar->p_half[i], (i ? sc1 : sc0) & 1, abort);
             if (ok && j == 0) ok = mbar_wait_warp(&bar->o_free[i], ((i ? ic1 : ic0) & 1) ^ 1, abort);
             if (!ok) break;
             tc_fence_after();
-            if (elect_one()) {
-              const uint64_t dv = desc_advance(dV, (kc & 1) * SM::kVBytes);
+            const uint64_t dv = desc_advance(dV, (kc & 1) * SM::kVBytes);
+            auto issue_pv = [&](uint32_t on, int k0) {
 #pragma unroll
-              for (int kk = 0; kk < kChN / 16; ++kk)
-                umma_ts(tmem + 256 + i * 128, tmem + i * 128 + kk * 8, desc_advance(dv, kk * 2048), idPV, (j > 0) || (kk > 0));
-              umma_commit(&bar->pv_done[i]);
-              if (i + 1 == ntile) umma_commit(&bar->v_empty[kc & 1]);
-            }
-            __syncwarp();
+              for (int kk = 0; kk < kChN / 32; ++kk)
+                mma_ts(on, tmem + 256 + i * 128, tmem + i * 128 + (k0 + kk) * 8, desc_advance(dv, (k0 + kk) * 2048), idPV, j > 0 || k0 + kk > 0);
+            };
+            by_leader([&](uint32_t on) { issue_pv(on, 0); });
+            ok = mbar_wait_warp(&bar->p_full[i], (i ? sc1 : sc0) & 1, abort);
+            if (!ok) break;
+            tc_fence_after();
+            by_leader([&](uint32_t on) {
+              issue_pv(on, kChN / 32);
+              commit(on, &bar->pv_done[i]);
+              if (i + 1 == ntile) commit(on, &bar->v_empty[kc & 1]);
+            });
             if (more) {
               if (i == 0) {
                 ok = mbar_wait_warp(&bar->k_full, (kc + 1) & 1, abort);
                 if (!ok) break;
                 tc_fence_after();
               }
-              if (elect_one()) {
-                issue_qk(i);
-                if (i + 1 == ntile) umma_commit(&bar->k_empty);
-              }
-              __syncwarp();
+              by_leader([&](uint32_t on) {
+                issue_qk(on, i);
+                if (i + 1 == ntile) commit(on, &bar->k_empty);
+              });
             }
             if (i) ++sc1; else ++sc0;
           }
@@ -521,6 +569,11 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
             sv[c][e] = h2u(__floats2half2_rn(p0, p1));
           }
           tmem_st32(tS + c * 16, sv[c]);
+          if (c == 0) {
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(&bar->p_half[i]);
+          }
         }
         l += rs[0] + rs[1];
         tc_wait_st();

@@ -4,8 +4,8 @@
 // A block of four warps has 16 rows of a kv group and walks the keys a page at a time, brought in by one bulk copy.  A warp forms the logits and
 // probabilities of one record (16 keys); through shared memory every warp gets all of them and forms the outputs of 32 value dimensions.
 // The cache's layout is the products' B fragment, so a chunk's codes come with one 8-byte load per lane.  (With keys and outputs of its own
-// for every warp there was no exchange, but 64 output registers a lane and a loop of 14 KB of instructions: 265 us where this takes 249, and
-// 28 where this takes 24 for the selected blocks of 32 tokens.)
+// for every warp there was no exchange, but 64 output registers a lane and a loop of 14 KB of instructions: 265 us where this took 249, and
+// 28 where this took 24 for the selected blocks of 32 tokens.)
 //
 // Logits: a nibble c masked out of its word where it lies is the fp16 number c 2^-24 (or 16 c 2^-24: the bits of a number below 2^-13 are its
 // multiple of 2^-24), so unpacking costs one AND per two codes; the sums start from -8 sum(q) 2^-24, which turns codes into values.  Each 32
@@ -15,7 +15,7 @@
 // Outputs: values times scales are exact in fp16; probabilities are rounded to fp16 (2^-11, an eighth of the output's own rounding).
 // The block's reference maximum of a row moves only when a row's maximum outgrows it by 2^8, so probabilities stay far below 65504.
 // Bound by instruction issue: about 480 instructions per 16 keys of a group, issued every second clock.  Without unpacking and products the same
-// loop takes 145 us for 64 requests of up to 32000 tokens (93 % of the copy bandwidth), with them 249.
+// loop takes 145 us for 64 requests of up to 32000 tokens (93 % of the copy bandwidth), with them 236.
 #include <algorithm>
 
 #include "attn_args.cuh"
