@@ -221,7 +221,8 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
       // ---------------------------------------------------------- MMA issuer (warp-uniform loops, one elected lane issues)
       // One lane issues.  Up to 128 key dimensions the whole warp walks through the instructions, each carried out by its leader, and the code of
       // either tile is its own: the descriptors of 16 products cost fewer instructions so (head dims 128/128, 2048 tokens behind 30000: 934 us
-      // against 1040 with a branch around them).  With 192 the branch and one copy of the code are faster: 2200 us against 2595.
+      // against 1040 with a branch around them; prompts of up to 1500 tokens, whose starts fetch more code, 155 against 152).  With 192 the
+      // branch and one copy of the code are faster: 2200 us against 2595.
       constexpr bool kBranch = DK > 128;
       constexpr int kCopies = kBranch ? 1 : 2;
       constexpr uint32_t idQK = idesc_f16(kChM, kChN, 0, 0), idPV = idesc_f16(kChM, DV, 0, 1);
