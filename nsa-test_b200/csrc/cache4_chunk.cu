@@ -473,20 +473,33 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar->piece_empty[c % kChPieces]);
     };
-    auto find = [&]() {                  // moves pc on to the next piece that has rows for this tile; false behind the last one
+    // Moves pc on to the next piece that has rows for this tile: 1 there is one, 0 there is none, -1 (not waiting) it is not known yet.  A warp
+    // that still has a piece's place must not wait for a later one: pieces without rows for its tile may fill all other places, and the
+    // one it waits for would need this one's.
+    auto find = [&](bool wait) {
       for (;; ++pc) {
-        if (!mbar_wait_warp(&bar->piece_full[pc % kChPieces], (pc / kChPieces) & 1, abort)) return false;
+        uint64_t* there = &bar->piece_full[pc % kChPieces];
+        const uint32_t parity = (pc / kChPieces) & 1;
+        if (wait) {
+          if (!mbar_wait_warp(there, parity, abort)) return 0;
+        } else if (!__all_sync(0xffffffffu, mbar_test(there, parity))) {
+          return -1;
+        }
         const ChunkPiece& w = bar->piece[pc % kChPieces];
-        if (w.n == 0 || i * kChM < w.nrows) return w.n > 0;
+        if (w.n == 0 || i * kChM < w.nrows) return w.n > 0 ? 1 : 0;
         release(pc);
       }
     };
-    bool more = find();
-    if (more) {
-      start_q(bar->piece[pc % kChPieces]);
-      finish_q();
-    }
-    while (more) {
+    int next = -1;
+    for (;;) {
+      if (next < 0) {                    // (no piece is held here)
+        next = find(true);
+        if (next > 0) {
+          start_q(bar->piece[pc % kChPieces]);
+          finish_q();
+        }
+      }
+      if (next <= 0) break;
       const int cur = pc;
       const ChunkPiece& s = bar->piece[cur % kChPieces];
       const int n = s.n, p0 = s.p0;
@@ -504,8 +517,8 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
         tc_fence_after();
         if (t + 1 == n) {
           ++pc;
-          more = find();
-          if (more) start_q(bar->piece[pc % kChPieces]);
+          next = find(false);
+          if (next > 0) start_q(bar->piece[pc % kChPieces]);
         }
         if (c0 < 0 || c1 < 0 || n0 + kChN - 1 > minpos || (a.window > 0 && n0 <= maxpos - a.window)) {
           int clo = a.window > 0 ? my_pos - a.window - n0 : -1, chi = my_pos - n0;       // visible columns: clo < c <= chi
@@ -584,7 +597,7 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
       if (!ok) break;
       const int last = (sc + n - 1) & 1;
       sc += n;
-      if (more) finish_q();
+      if (next > 0) finish_q();
       ok = mbar_wait_warp(&bar->pv_done[i], last, abort);
       if (!ok) break;
       tc_fence_after();

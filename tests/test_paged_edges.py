@@ -1,0 +1,82 @@
+"""Paged serving where it can go wrong: many short requests, queries and lengths beyond the ordinary, steps taken apart."""
+import math
+import random
+
+import pytest
+import torch
+
+from tests import paged_ref as ref
+from tests.test_paged import BF, F32, HEADS, ODD_HEADS, Served
+
+
+def by_request(s, q, lengths=None, scale=None, window=None):
+    """``ref.attend`` for all tokens of a request and group at once (64 bits): o, L, M, A, B, V."""
+    q, N, H = q.double(), q.shape[0], q.shape[1]
+    G, dk, dv = s.k[0].shape[1], s.dk, s.v[0].shape[2]
+    hp, scale = H // G, s.dk ** -0.5 if scale is None else scale
+    o = torch.full((N, H, dv), math.nan, dtype=torch.float64, device=q.device)
+    A, V, L = o.clone(), o.clone(), o[..., 0].clone()
+    M, B = L.clone(), L.clone()
+    for r, length in enumerate(s.lengths if lengths is None else lengths):
+        a, b = s.starts[r], s.starts[r + 1]
+        if a == b:
+            continue
+        j = torch.arange(length, device=q.device)
+        pos = length - b + torch.arange(a, b, device=q.device)
+        see = j <= pos[:, None]
+        if window is not None:
+            see &= j > pos[:, None] - window
+        for g in range(G):
+            at = (slice(a, b), slice(g * hp, (g + 1) * hp))
+            k, v = s.k[r][:length, g].double(), s.v[r][:length, g].double()
+            mask = lambda x, y: torch.where(see[:, None], x, torch.full_like(x, y))
+            x = mask(q[at] @ k.T * scale, -math.inf)
+            M[at] = x.amax(-1)
+            p = torch.exp(x - M[at][..., None])
+            l = p.sum(-1, keepdim=True)
+            o[at], A[at], L[at] = p @ v / l, p @ v.abs() / l, torch.log(l[..., 0])
+            B[at] = mask(q[at].abs() @ k.abs().T * abs(scale), 0.0).amax(-1)
+            V[at] = (see.double() @ v.abs())[:, None].expand(-1, hp, -1)
+    return o, L, M, A, B, V
+
+
+# ------------------------------------------------------------------------------------------------ many short requests
+
+def _rows(hp, *rows):
+    """New tokens that make so many rows (token, head) of a group, rounded up."""
+    return [-(-r // hp) for r in rows]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("pattern", [(160, 96), (256, 80, 128, 96, 80), (96, 80, 128, 256), (300, 90, 90, 90, 90, 90), None])
+@pytest.mark.parametrize("window", [None, 30])
+def test_many_pieces_a_block(heads, pattern, window):
+    """Hundreds of short requests: a block has more of them than it holds at once, with one row tile or two in any order."""
+    hp = heads[0] // heads[1]
+    rng = random.Random(30)
+    S = 1200 // heads[1]
+    rows = [rng.choice([80, 96, 128, 129, 200, 256, 257, 400]) for _ in range(S)] if pattern is None else [pattern[i % len(pattern)] for i in range(S)]
+    new = _rows(hp, *rows)
+    s = Served([n + rng.choice([0, 1, rng.randint(0, 150)]) for n in new], new, *heads, BF, seed=30)
+    got = s.cache.attend(s.q, s.table, s.len_dev, s.starts_dev, window=window)
+    ref.check(got, by_request(s, s.q, window=window), BF, max(s.lengths), s.dk)
+    for _ in range(5):
+        again = s.cache.attend(s.q, s.table, s.len_dev, s.starts_dev, window=window)
+        assert all(torch.equal(x, y) for x, y in zip(got, again))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("every", [3, 5, 9, 1000])
+def test_a_padded_step_of_mostly_single_tokens(heads, every):
+    """Room for 256 rows a request, of which most bring one token: all are one kernel's, and most pieces have one row tile."""
+    hp, S = heads[0] // heads[1], 1000 // heads[1]
+    most = 256 // hp
+    rng = random.Random(every)
+    new = [most if i % every == 0 else rng.choice([1, 1, 1, 2]) for i in range(S)]
+    s = Served([n + rng.randint(0, 200) for n in new], new, *heads, BF, seed=31)
+    N = s.starts[-1]
+    q = torch.cat((s.q, s.q.new_full((S * most - N, *s.q.shape[1:]), math.nan)))
+    o, L, M = s.cache.attend(q, s.table, s.len_dev, s.starts_dev, max_new=most)
+    ref.check((o[:N], L[:N], M[:N]), by_request(s, s.q), BF, max(s.lengths), s.dk)
