@@ -45,7 +45,8 @@ struct FmaCore {
     for (int i = threadIdx.x; i < RT * a.dk; i += kC4Threads) {
       const int r = i / a.dk, d = i - r * a.dk, f = s.row0 + r;
       float x = 0.f;
-      if (r < s.nrows) x = Elem<T>::ld((const T*)a.q + (s.tok0 + f / a.hpg) * a.sq_tok + (s.g * a.hpg + f % a.hpg) * a.sq_head + d) * a.scale;
+      if (r < s.nrows) x = Elem<T>::ld((const T*)a.q + (s.tok0 + f / a.hpg) * a.sq_tok + (s.g * a.hpg + f % a.hpg) * a.sq_head + d);
+      x = isfinite(x) ? x * a.scale : CUDART_NAN_F;
       qs[i] = x;
     }
 #pragma unroll
@@ -95,7 +96,7 @@ struct FmaCore {
       if (at > pos || (a.window > 0 && at <= pos - a.window)) x[r] = -CUDART_INF_F;
       const float mx = fmaxf(m[r], warp_max(x[r]));
       f[r] = m[r] == mx ? 1.f : ex2((m[r] - mx) * kLog2e);
-      const float pr = mx == -CUDART_INF_F ? 0.f : ex2((x[r] - mx) * kLog2e);
+      const float pr = x[r] == -CUDART_INF_F ? 0.f : ex2((x[r] - mx) * kLog2e);
       m[r] = mx;
       l[r] = l[r] * f[r] + warp_sum(lane < 16 ? pr : 0.f);
       if (lane < 16) p[r * 16 + place] = pr;
@@ -243,12 +244,12 @@ __global__ void __launch_bounds__(kC4Threads, Core::kBlocksPerSm) cache4_attn_ke
         const int64_t row = out_row(a, s, r);
         Elem<T>::st((T*)a.out + row * a.dv + d, l > 0.f ? x / l : x);
         if (d == 0) {
-          a.M[row] = m;
+          a.M[row] = max_of_row(m, l);
           a.L[row] = logf(l);
         }
       } else {
         part[i] = x;
-        if (d == 0) reinterpret_cast<float2*>(part + ROWS * a.dv)[r] = make_float2(m, l);
+        if (d == 0) reinterpret_cast<float2*>(part + ROWS * a.dv)[r] = make_float2(max_of_row(m, l), l);
       }
     }
     if (!whole && place == 0)
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(128) cache4_combine_kernel(const Cache4Args a,
     float2 h = make_float2(-CUDART_INF_F, 0.f);
     if (p < rec.pieces) h = reinterpret_cast<const float2*>(part(p) + rows * a.dv)[r];
     const float mx = fmaxf(m, warp_max(h.x));
-    if (mx == -CUDART_INF_F) continue;
+    if (mx == -CUDART_INF_F && !__any_sync(0xffffffffu, h.x != h.x)) continue;      // (a row that is NaN goes on, whatever the maximum)
     const float f = ex2((m - mx) * kLog2e), w = ex2((h.x - mx) * kLog2e);
     m = mx;
     l = l * f + warp_sum(h.y * w);
@@ -344,7 +345,7 @@ __global__ void __launch_bounds__(128) cache4_combine_kernel(const Cache4Args a,
       Elem<T>::st(to, x[i].x * inv); Elem<T>::st(to + 1, x[i].y * inv); Elem<T>::st(to + 2, x[i].z * inv); Elem<T>::st(to + 3, x[i].w * inv);
     }
   if (lane == 0) {
-    a.M[row] = m;
+    a.M[row] = max_of_row(m, l);
     a.L[row] = logf(l);
   }
 }

@@ -305,6 +305,10 @@ __device__ __forceinline__ float* split_part(const Cache4Args& a, int blocks, in
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// A query row with a NaN or an infinity has no softmax: it is NaN from the start (each kernel's), so are all its logits and the sum of its
+// probabilities.  The maximum is not (the larger of a number and NaN is the number) and follows here, or the row would pass for one that sees nothing.
+__device__ __forceinline__ float max_of_row(float m, float l) { return l == l ? m : CUDART_NAN_F; }
+
 // row i of a segment: its token and head
 __device__ __forceinline__ int64_t out_row(const Cache4Args& a, const Segment& s, int i) {
   const int f = s.row0 + i;

@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
       mx = max(mx & 0xffffu, mx >> 16);
       const int k = mx ? min(14 - ((int)(mx >> 7) - 127), 100) : 0;
       // the scale's sign goes into the row, so that larger S is always the larger logit; scale 0 is a row of zeros
-      const float up = __uint_as_float((uint32_t)(k + 127) << 23) * (a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f);
+      const float up = mx >= 0x7f80 ? CUDART_NAN_F : __uint_as_float((uint32_t)(k + 127) << 23) * (a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f);
       cl = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * __uint_as_float((uint32_t)(127 - k) << 23);
       pos = pos_next;
 #pragma unroll 2
@@ -654,7 +654,7 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
         }
       }
       if (row < s.nrows) {
-        const float M = m_true == -CUDART_INF_F ? m_true : m_true * row_cl;
+        const float M = max_of_row(m_true == -CUDART_INF_F ? m_true : m_true * row_cl, l);
         if (s.whole) {
           a.M[orow] = M;
           a.L[orow] = logf(l * rel);

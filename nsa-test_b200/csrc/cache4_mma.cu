@@ -92,7 +92,7 @@ __device__ __forceinline__ void load_rows(const Cache4Args& a, const Segment& s,
     mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     const int k = mx ? min(14 - ((int)(mx >> 7) - 127), 100) : 0;
     // the scale's sign goes into the row, so that a larger sum is always the larger logit; scale 0 is a row of zeros
-    up[h] = __uint_as_float((uint32_t)(k + 127) << 23) * (a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f);
+    up[h] = mx >= 0x7f80 ? CUDART_NAN_F : __uint_as_float((uint32_t)(k + 127) << 23) * (a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f);
     st.cl[h] = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * __uint_as_float((uint32_t)(127 - k) << 23) * 16777216.f;
     st.c2[h] = st.cl[h] * kLog2e;
     st.m[h] = st.lim[h] = st.top[h] = -CUDART_INF_F;
@@ -405,8 +405,8 @@ __global__ void __launch_bounds__(kMmThreads, MmaSmem<GK, GV>::kBlocksPerSm) cac
         const int r = n + 8 * h;
         if (r >= s.nrows) continue;
         const float2 h0 = ml[0][r], h1 = ml[1][r], h2 = ml[2][r], h3 = ml[3][r];
-        top[h] = fmaxf(fmaxf(h0.x, h1.x), fmaxf(h2.x, h3.x));
         sum[h] = (h0.y + h1.y) + (h2.y + h3.y);
+        top[h] = max_of_row(fmaxf(fmaxf(h0.x, h1.x), fmaxf(h2.x, h3.x)), sum[h]);
         const float rel = top[h] == -CUDART_INF_F ? 0.f : ex2((st.m[h] - top[h]) * st.c2[h]);       // to the row's true maximum
         const float M = top[h] == -CUDART_INF_F ? top[h] : top[h] * st.cl[h];
         f[h] = whole ? (sum[h] > 0.f ? 1.f / sum[h] : sum[h]) : rel;

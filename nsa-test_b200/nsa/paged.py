@@ -126,8 +126,8 @@ class PagedCache4:
         (their own among them) are in the cache under ``table [S,P]``, ``lengths [S]``.  Each sees the keys up to its own position;
         with ``window`` the last so many of them; with ``indices [N,G,n]`` (int32, n <= 32) those in the named 64-key blocks of its request,
         negative entries and repetitions not counting.  -> (o ``[N,H,dv]`` in the type of q, L, M ``[N,H]`` fp32: log sum and maximum of
-        the logits, as of the other branches); rows that see nothing are 0 with L = M = -inf, rows behind the last request's
-        stay as they were.  ``max_new``: a bound of the requests' numbers of new tokens, where the host knows one.
+        the logits, as of the other branches); rows that see nothing are 0 with L = M = -inf, rows that see something with a query that holds a
+        NaN or an infinity are NaN in all three, rows behind the last request's stay as they were.  ``max_new``: a bound of the requests' numbers of new tokens, where the host knows one.
         """
         dk, dv, G = self.head_dim_qk, self.head_dim_v, self.storage.shape[1]
         if q.dim() != 3 or q.shape[2] != dk or q.shape[1] % G or q.shape[1] == 0:

@@ -80,3 +80,49 @@ def test_a_padded_step_of_mostly_single_tokens(heads, every):
     q = torch.cat((s.q, s.q.new_full((S * most - N, *s.q.shape[1:]), math.nan)))
     o, L, M = s.cache.attend(q, s.table, s.len_dev, s.starts_dev, max_new=most)
     ref.check((o[:N], L[:N], M[:N]), by_request(s, s.q), BF, max(s.lengths), s.dk)
+
+
+# ------------------------------------------------------------------------------------------------ queries beyond the ordinary
+
+# (lengths, new tokens): segments that one block has whole, segments that many blocks share, several row tiles, prompts
+LAYOUTS = [([40, 7, 64], [1, 1, 1]), ([20000, 5], [1, 1]), ([90, 3000, 33], [3, 2, 4]), ([150, 40, 60], [150, 40, 60]), ([6000], [40])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,heads", [(BF, HEADS[0]), (BF, HEADS[1]), (BF, HEADS[2]), (F32, HEADS[2]), (BF, ODD_HEADS[0])])
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("form", ["all", "window", "selected"])
+def test_rows_that_are_not_finite(dtype, heads, layout, form):
+    """A NaN or an infinity in a query makes that row NaN however the work is cut, and no other row anything else."""
+    s = Served(*layout, *heads, dtype, seed=32)
+    N, H, dk = s.q.shape
+    kw = dict(window=dict(window=33), all={}, selected=dict(indices=torch.randint(0, -(-min(s.lengths) // 64), (N, heads[1], 3), dtype=torch.int32).cuda()))[form]
+    clean = s.q.clone()
+    rng = random.Random(33)
+    bad = torch.zeros(N, H, dtype=torch.bool, device="cuda")
+    for _ in range(min(5, N * H // 2)):
+        i, h = rng.randrange(N), rng.randrange(H)
+        bad[i, h] = True
+        clean[i, h] = 0
+        what = rng.choice([math.nan, math.inf, -math.inf])
+        if rng.random() < 0.3:
+            s.q[i, h] = what
+        else:
+            s.q[i, h, rng.randrange(dk)] = what
+    got = s.cache.attend(s.q, s.table, s.len_dev, s.starts_dev, **kw)
+    want = s.cache.attend(clean, s.table, s.len_dev, s.starts_dev, **kw)
+    assert want[0].isfinite().all()
+    blind = want[2] == -math.inf                    # (a row may see nothing of the named blocks: then its query does not count)
+    for x, y in zip(got, want):
+        assert x[bad & ~blind].isnan().all() and torch.equal(x[~bad | blind], y[~bad | blind])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("new", [1, 40])
+def test_rows_that_are_not_finite_and_see_nothing(dtype, new):
+    s = Served([200, 90], [new, 1], *HEADS[2], dtype, seed=34)
+    s.q[0] = math.nan
+    s.table[:] = -1
+    o, L, M = s.cache.attend(s.q, s.table, s.len_dev, s.starts_dev)
+    assert not o.any() and (L == -math.inf).all() and (M == -math.inf).all()
