@@ -159,10 +159,10 @@ __global__ void __launch_bounds__(kC4Threads, Core::kBlocksPerSm) cache4_attn_ke
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int groups = (a.dk + a.dv) / kGroupDims, rec_bytes = groups * kRecBytesPerGroup;
   uint8_t* ring = smem + warp * kC4Stages * rec_bytes;
-  uint8_t* extra = smem + max(kC4Warps * kC4Stages * rec_bytes, 4096 * 4);
+  uint8_t* extra = smem + max(kC4Warps * kC4Stages * rec_bytes, kHeldBytes);
 
   Walk<ROWS, kPageTokens, 1, true> walk(a);
-  int* held = reinterpret_cast<int*>(smem);
+  long long* held = reinterpret_cast<long long*>(smem);
   walk.template start<kC4Threads>(scratch, held);
   long long u = share(walk.total, blockIdx.x, gridDim.x);
   const long long end = share(walk.total, blockIdx.x + 1, gridDim.x);
@@ -380,7 +380,7 @@ constexpr int kChunkRows = 80;
 
 // records in flight; at first the requests' units are held there
 static size_t ring_bytes(int dk, int dv) {
-  return std::max<size_t>((size_t)kC4Warps * kC4Stages * ((dk + dv) / kGroupDims) * kRecBytesPerGroup, 4096 * 4);
+  return std::max<size_t>((size_t)kC4Warps * kC4Stages * ((dk + dv) / kGroupDims) * kRecBytesPerGroup, kHeldBytes);
 }
 
 int cache4_grid(const Cache4Args& a, int rows, int per_sm) {

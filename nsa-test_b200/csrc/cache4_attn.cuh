@@ -14,6 +14,9 @@ namespace nsa {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kSelMax = 32;          // places of a block list: one per lane
+// Requests whose units are held in shared memory at once.  A unit number has 64 bits: rows in tiles of 8 times up to 2^23 pages, a prompt
+// of 371 000 tokens with 16 heads a group has 2^31 of them already.
+constexpr int kHeldRequests = 4096, kHeldBytes = kHeldRequests * 8;
 
 struct Segment {
   int tok0;        // first token of the request among the step's (selected form: the token)
@@ -49,7 +52,7 @@ __device__ __forceinline__ int block_of(long long total, long long u, int n) {
 // SEL: the selected form can be asked for.
 template <int ROWS, int KEYS, int OVER, bool SEL>
 struct Walk {
-  static constexpr int kChunk = 4096;       // requests whose units are held in shared memory at once
+  static constexpr int kChunk = kHeldRequests;
   const Cache4Args& a;
   Segment s;
   int tile, tiles, len, fresh;              // of the current request
@@ -112,11 +115,12 @@ struct Walk {
   // units (of one group) of requests base .. base + kChunk - 1 into shared memory: a thread per request, or where a request has many
   // tiles a warp
   template <int T>
-  __device__ __forceinline__ void fill(int base, int* held) const {
+  __device__ __forceinline__ void fill(int base, long long* held) const {
     const int n = min(kChunk, a.S - base), lane = threadIdx.x & 31;
     if ((long long)a.N * a.hpg <= 4ll * ROWS * a.S) {
       for (int i = threadIdx.x; i < n; i += T) {
-        int tok0, fresh, length, sum = 0;
+        int tok0, fresh, length;
+        long long sum = 0;
         request(base + i, tok0, fresh, length);
         for (int t = 0, m = row_tiles(fresh); t < m; ++t) {
           int lo, hi;
@@ -127,7 +131,8 @@ struct Walk {
       }
     } else {
       for (int i = threadIdx.x >> 5; i < n; i += T / 32) {
-        int tok0, fresh, length, sum = 0;
+        int tok0, fresh, length;
+        long long sum = 0;
         request(base + i, tok0, fresh, length);
         for (int t = lane, m = row_tiles(fresh); t < m; t += 32) {
           int lo, hi;
@@ -142,9 +147,9 @@ struct Walk {
     __syncthreads();
   }
 
-  // Number of all units; all T threads of the block take part.  scratch: T / 32 + 3 long longs of shared memory, held: kChunk ints.
+  // Number of all units; all T threads of the block take part.  scratch: T / 32 + 3 long longs of shared memory, held: kHeldBytes of it.
   template <int T>
-  __device__ __forceinline__ void start(long long* scratch, int* held) {
+  __device__ __forceinline__ void start(long long* scratch, long long* held) {
     if (SEL && a.n_sel) {
       const int n = min(max(a.starts[a.S], 0), a.N);
       tiles = (a.hpg + ROWS - 1) / ROWS;
@@ -170,7 +175,7 @@ struct Walk {
   }
   // Segment that unit u (< total) lies in; returns its place within the segment.
   template <int T>
-  __device__ __forceinline__ int seek(long long u, long long* scratch, int* held) {
+  __device__ __forceinline__ int seek(long long u, long long* scratch, long long* held) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (SEL && a.n_sel) {
       const long long seg = quotient(u, length()), of_tiles = quotient(seg, tiles), of_groups = quotient(of_tiles, a.G);
@@ -199,7 +204,7 @@ struct Walk {
       }
       for (int i0 = 0; i0 < min(kChunk, a.S - base) && !found; i0 += T) {
         const int i = i0 + threadIdx.x;
-        const long long x = i < min(kChunk, a.S - base) ? (long long)held[i] * a.G : 0;
+        const long long x = i < min(kChunk, a.S - base) ? held[i] * a.G : 0;
         long long p = x;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -229,7 +234,7 @@ struct Walk {
     const long long off = scratch[T / 32 + 1], per = scratch[T / 32 + 2];
     __syncthreads();
     s.g = (int)quotient(off, per);
-    int place = (int)(off - s.g * per);
+    long long place = off - s.g * per;
     for (int t0 = 0;; t0 += 32) {               // 32 tiles at a time
       int lo, hi, p = 0;
       if (t0 + lane < tiles) {
@@ -247,7 +252,7 @@ struct Walk {
         if (k > 0) place -= __shfl_sync(0xffffffffu, p, k - 1);
         tile = t0 + k;
         set_tile();
-        return place;
+        return (int)place;
       }
       place -= __shfl_sync(0xffffffffu, p, 31);
     }
@@ -255,7 +260,7 @@ struct Walk {
   // Unit at which block c's share begins.  A boundary inside a segment that is short against a share moves to the segment's nearer end: what
   // such a segment would cost as two partial results is more than the shares then differ by.  Leaves the walk at that unit, its place in `place`.
   template <int T>
-  __device__ __forceinline__ long long boundary(int c, int n, long long* scratch, int* held, int& place) {
+  __device__ __forceinline__ long long boundary(int c, int n, long long* scratch, long long* held, int& place) {
     long long u = share(total, c, n);
     place = 0;
     if (u >= total) return u;

@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
   const uint32_t tmem = bar->tmem_base;
 
   Walk<kChRows, kChN, kChOver, false> walk(a);
-  int* held = reinterpret_cast<int*>(smem);       // where queries will be
+  long long* held = reinterpret_cast<long long*>(smem);       // where queries will be
   walk.template start<kChThreads>(bar->scratch, held);
   // once any block has given up on a wait the device's results are void: later blocks skip their work
   if (threadIdx.x == 0) bar->scratch[0] = *(volatile const int*)timeouts != 0 ? 0 : walk.total;

@@ -36,8 +36,8 @@ constexpr float kMmGrow = 8.f;                       // log2 units
 template <int GK, int GV>
 struct MmaSmem {
   static constexpr int kRecBytes = (GK + GV) * kRecBytesPerGroup, kStageBytes = kRecsPerPage * kRecBytes, kRingBytes = kMmStages * kStageBytes;
-  static constexpr int kHeld = 4096 * 4;               // the requests' units, at first
-  static constexpr int oQ = kRingBytes > kHeld ? kRingBytes : kHeld, oC = oQ + GK * 1024, oP = oC + GK * 128, kDynamic = oP + 2 * 2048;
+  static constexpr int oQ = kRingBytes > kHeldBytes ? kRingBytes : kHeldBytes,       // (the requests' units are there at first)
+                        oC = oQ + GK * 1024, oP = oC + GK * 128, kDynamic = oP + 2 * 2048;
   static constexpr int kBlocksPerSm = 4;
 };
 
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(kMmThreads, MmaSmem<GK, GV>::kBlocksPerSm) cac
   __shared__ typename W::Place at_place;
   {
     W walk(a);
-    int* held = reinterpret_cast<int*>(smem);
+    long long* held = reinterpret_cast<long long*>(smem);
     walk.template start<kMmThreads>(scratch, held);
     if (__syncthreads_or(gave_up)) walk.total = 0;
     const long long u = share(walk.total, blockIdx.x, gridDim.x), end = share(walk.total, blockIdx.x + 1, gridDim.x);

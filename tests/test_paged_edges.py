@@ -9,8 +9,8 @@ from tests import paged_ref as ref
 from tests.test_paged import BF, F32, HEADS, ODD_HEADS, Served
 
 
-def by_request(s, q, lengths=None, scale=None, window=None):
-    """``ref.attend`` for all tokens of a request and group at once (64 bits): o, L, M, A, B, V."""
+def by_request(s, q, lengths=None, scale=None, window=None, held=None):
+    """``ref.attend`` for all tokens of a request and group at once (64 bits): o, L, M, A, B, V.  held[r]: the positions of keys s.k[r], where not all are there."""
     q, N, H = q.double(), q.shape[0], q.shape[1]
     G, dk, dv = s.k[0].shape[1], s.dk, s.v[0].shape[2]
     hp, scale = H // G, s.dk ** -0.5 if scale is None else scale
@@ -21,14 +21,14 @@ def by_request(s, q, lengths=None, scale=None, window=None):
         a, b = s.starts[r], s.starts[r + 1]
         if a == b:
             continue
-        j = torch.arange(length, device=q.device)
+        j = torch.arange(length, device=q.device) if held is None else held[r]
         pos = length - b + torch.arange(a, b, device=q.device)
         see = j <= pos[:, None]
         if window is not None:
             see &= j > pos[:, None] - window
         for g in range(G):
             at = (slice(a, b), slice(g * hp, (g + 1) * hp))
-            k, v = s.k[r][:length, g].double(), s.v[r][:length, g].double()
+            k, v = s.k[r][:len(j), g].double(), s.v[r][:len(j), g].double()
             mask = lambda x, y: torch.where(see[:, None], x, torch.full_like(x, y))
             x = mask(q[at] @ k.T * scale, -math.inf)
             M[at] = x.amax(-1)
@@ -126,3 +126,38 @@ def test_rows_that_are_not_finite_and_see_nothing(dtype, new):
     s.table[:] = -1
     o, L, M = s.cache.attend(s.q, s.table, s.len_dev, s.starts_dev)
     assert not o.any() and (L == -math.inf).all() and (M == -math.inf).all()
+
+
+# ------------------------------------------------------------------------------------------------ more units than 32 bits count
+
+@pytest.mark.gpu
+def test_more_units_of_work_than_32_bits_count():
+    """The longest table there may be, with six pages in it: 320 row tiles of 8 388 608 pages are 2.7e9 units of work, behind and in front of
+    requests of a page."""
+    from types import SimpleNamespace
+
+    from nsa.paged import PagedCache4
+    H, dk, P, new = 16, 32, 1 << 23, [1, 160, 2]
+    lengths = [60, P * 64, 40]
+    pages = {0: [0], 1: [0, 1, P // 2, P - 3, P - 2, P - 1], 2: [0]}
+    table = torch.full((3, P), -1, dtype=torch.int32, device="cuda")
+    c = PagedCache4.empty(8, 1, dk, dk)
+    s = SimpleNamespace(lengths=lengths, starts=[0, 1, 161, 163], dk=dk, k=[], v=[])
+    gen = torch.Generator(device="cuda").manual_seed(40)
+    rn = lambda *shape: torch.randn(*shape, generator=gen, device="cuda")
+    held, at = [], 0
+    for r in range(3):
+        ids = torch.arange(at, at + len(pages[r]), device="cuda")
+        at += len(pages[r])
+        table[r, torch.tensor(pages[r], device="cuda")] = ids.int()
+        slots = (ids[:, None] * 64 + torch.arange(64, device="cuda")).view(-1)
+        c.append(rn(len(slots), 1, dk), rn(len(slots), 1, dk), slots)
+        k, v = c.read(slots)
+        s.k.append(k)
+        s.v.append(v)
+        held.append((torch.tensor(pages[r], device="cuda")[:, None] * 64 + torch.arange(64, device="cuda")).view(-1))
+    q = rn(163, H, dk)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    got = c.attend(q, table, i32(lengths), i32(s.starts))
+    # 384 keys and at most 296 partial results a row
+    ref.check(got, by_request(s, q, held=held), F32, 1000, dk)
