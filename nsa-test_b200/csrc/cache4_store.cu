@@ -18,9 +18,11 @@ struct TablesArgs {
   int S, P, F, N, page;
 };
 
-// Lengths and sums of them are held below 2^30, whatever the caller's numbers: no index derived from them leaves 32 bits.
+// Lengths are held to 2^29 and sums of them below 2^30, whatever the caller's numbers.  So two sums add up within 32 bits, a sum is never less
+// than its last term, and (first_tok[0] being 0) a token's request starts at or before it: positions, and page numbers in a row or on the
+// free list, are not negative.
 __device__ __forceinline__ int bounded(int x) { return min(max(x, 0), 1 << 29); }
-__device__ __forceinline__ int add(int x, int y) { return min(x + y, 1 << 30); }
+__device__ __forceinline__ int add(int x, int y) { return min(x + y, (1 << 30) - 1); }
 
 // Every block forms the prefix sums of all requests' new tokens and new pages (8 bytes a request out of L2, far less than what a
 // second launch or a wait between blocks costs), then deals with its own 512 tokens.  A token whose position opens a page takes
@@ -63,8 +65,8 @@ __global__ void __launch_bounds__(kTblMaxThreads) block_tables_kernel(const Tabl
       run.y = add(run.y, t.y);
     }
     if (r < a.S) {
-      first_tok[r] = before.x + s.x - x.x;
-      first_page[r] = before.y + s.y - x.y;
+      first_tok[r] = add(before.x, s.x) - x.x;
+      first_page[r] = add(before.y, s.y) - x.y;
       if (blockIdx.x == 0) {
         a.starts[r] = first_tok[r];
         a.lengths[r] = len;
@@ -98,8 +100,8 @@ __global__ void __launch_bounds__(kTblMaxThreads) block_tables_kernel(const Tabl
       if (pi < have) {
         id = a.table[(int64_t)r * a.table_ld + pi];
       } else {
-        const int at = first_page[r] + pi - have;
-        id = at < a.F ? a.free_pages[at] : -1;
+        const unsigned at = (unsigned)first_page[r] + (unsigned)(pi - have);      // (below 2^30 + 2^29 + 2^30)
+        id = at < (unsigned)a.F ? a.free_pages[at] : -1;
         if (off == 0) a.table[(int64_t)r * a.table_ld + pi] = id;
       }
     }

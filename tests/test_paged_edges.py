@@ -161,3 +161,95 @@ def test_more_units_of_work_than_32_bits_count():
     got = c.attend(q, table, i32(lengths), i32(s.starts))
     # 384 keys and at most 296 partial results a row
     ref.check(got, by_request(s, q, held=held), F32, 1000, dk)
+
+
+# ------------------------------------------------------------------------------------------------ block tables of lengths beyond reason
+
+LIMIT = 2 ** 30 - 1
+
+
+def _bounded_tables(cached, new, table, free, tokens, page):
+    """slots and positions as nsa_block_tables finds them, sums of lengths held below 2^30: every page it reads or writes is one of its own."""
+    hold = lambda x: min(max(x, 0), 2 ** 29)
+    c, n = [hold(x) for x in cached], [hold(x) for x in new]
+    have = [-(-x // page) for x in c]
+    need = [-(-(x + y) // page) - h for x, y, h in zip(c, n, have)]
+    first, opened, taken, t = [], [], 0, 0
+    for x, y in zip(n, need):
+        t, taken = min(t + x, LIMIT), min(taken + y, LIMIT)
+        first.append(t - x)
+        opened.append(taken - y)
+    table = [list(r) for r in table]
+    rows = []
+    for i in range(min(tokens, t)):
+        r, up = 0, len(c)
+        while up - r > 1:
+            mid = (r + up) // 2
+            r, up = (mid, up) if first[mid] <= i else (r, mid)
+        pos = c[r] + i - first[r]
+        at = pos // page
+        assert pos >= 0 and first[r] >= 0 and opened[r] >= 0
+        rows.append((r, pos, at, opened[r] + at - have[r] if at >= have[r] else None))
+    before = [list(x) for x in table]
+    for r, pos, at, f in rows:
+        if at < len(table[r]) and f is not None and pos % page == 0:
+            table[r][at] = free[f] if f < len(free) else -1
+    slots, positions = [], []
+    for r, pos, at, f in rows:
+        id = -1
+        if at < len(table[r]):
+            id = before[r][at] if f is None else free[f] if f < len(free) else -1
+        slots.append(id * page + pos % page if id >= 0 else -1)
+        positions.append(pos)
+    pad = [-1] * (tokens - len(rows))
+    return table, slots + pad, positions + pad, first + [t], [x + y for x, y in zip(c, n)], taken
+
+
+def _wild_lengths(S, seed):
+    rng = random.Random(seed)
+    some = [0, 0, 1, 5, 2 ** 29, 2 ** 30, 2 ** 31 - 1, -1, -2 ** 31, rng.randint(0, 2 ** 31 - 1)]
+    if seed == 0:
+        return [0] * S, [2 ** 29] * S
+    if seed == 1:                                   # sums at their limit, then requests without tokens
+        return [0] * S, [2 ** 31 - 1 if i < S * 3 // 4 else 0 for i in range(S)]
+    if seed == 2:
+        return [2 ** 31 - 1] * S, [70 if i == 0 else rng.choice(some) for i in range(S)]
+    return [rng.choice(some) for _ in range(S)], [rng.choice(some) for _ in range(S)]
+
+
+def _wrapping_lengths(seed):
+    """(Sums of these that wrap around 32 bits would give a token of theirs a page number below zero.)"""
+    rng = random.Random(seed)
+    S = rng.choice([5, 6, 8, 9, 12, 40])
+    return [rng.choice([0, 0, 100, 2 ** 29]) for _ in range(S)], [rng.choice([0, 1, 2 ** 29, 2 ** 29, 2 ** 31 - 1, 5]) for _ in range(S)]
+
+
+def _check_bounded(c, n, page, tokens):
+    """No entry outside the table and the free list is read or written."""
+    from nsa.paged import block_tables
+    S, P = len(c), 5
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    around = torch.full((S + 2000, P), 12345678, dtype=torch.int32, device="cuda")       # an entry of it would give itself away
+    table = around[1000:1000 + S]
+    host = [[r * P + i for i in range(P)] for r in range(S)]
+    table.copy_(i32(host))
+    free = list(range(100000, 100050))
+    want = _bounded_tables(c, n, host, free, tokens, page)
+    step = block_tables(i32(c), i32(n), table, i32(free), tokens, page)
+    assert table.tolist() == want[0]
+    assert [x.tolist() for x in step[:4]] == [want[1], want[2], want[3], want[4]] and step.pages.tolist() == [want[5]]
+    assert (around[:1000] == 12345678).all() and (around[1000 + S:] == 12345678).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [4, 40, 300, 1100])
+@pytest.mark.parametrize("page", [1, 64, 65536])
+@pytest.mark.parametrize("seed", [0, 1, 2, 3, 4])
+def test_block_tables_of_lengths_beyond_reason(S, page, seed):
+    _check_bounded(*_wild_lengths(S, 5 * seed + S if seed > 2 else seed), page, 2000)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", [27, 1171, 1241, 1892, 1958])
+def test_block_tables_of_sums_that_would_wrap(seed):
+    _check_bounded(*_wrapping_lengths(seed), 64, 64)
