@@ -18,6 +18,10 @@ constexpr int kSelMax = 32;          // places of a block list: one per lane
 // of 371 000 tokens with 16 heads a group has 2^31 of them already.
 constexpr int kHeldRequests = 4096, kHeldBytes = kHeldRequests * 8;
 
+// Probabilities that become fp16 are 2^7 times what they are against a row's reference: the reference lags by 2^8 at most, so they stay below
+// 65504, and fp16 ends at 2^-32 of the reference instead of 2^-25.  (Sums have the factor too; results take it out.)
+constexpr float kProbShift = 7.f, kProbUnshift = 0.0078125f;
+
 struct Segment {
   int tok0;        // first token of the request among the step's (selected form: the token)
   int row0, nrows; // first flattened row (token * heads per group + head) within the request and how many there are

@@ -6,8 +6,9 @@
 //   warps 8-11       unpack a tile's keys and values out of L2 into shared memory: fp16 holds (c - 8) s exactly
 //   warp 13          walks the block's segments and hands the pieces to the others
 //   warp 12          issues the MMAs: S_i = Q_i K^T (both operands in shared memory), O_i += P_i V (P in tensor memory)
-// TMEM columns and the order PV0(j) QK0(j+1) PV1(j) QK1(j+1) are those of the dense forward kernel.  Probabilities are rounded to fp16 (2^-11);
-// those of the first 64 keys are handed over while the others are formed (head dims 128/128: 1080 -> 1035 us, 192/128: no change).
+// TMEM columns and the order PV0(j) QK0(j+1) PV1(j) QK1(j+1) are those of the dense forward kernel.  Probabilities are rounded to fp16:
+// by 2^-11 down to 2^-21 of the row's reference, by 2^-32 of the reference below (kProbShift).  Those of the first 64 keys are handed over while
+// the others are formed (head dims 128/128: 1080 -> 1035 us, 192/128: no change).
 //
 // Where a code lies in its word fixes in which order a thread unpacks it for free; the two operands of a product only have to agree.  So
 // eight dimensions of a query and a key lie in the order 0 4 1 5 2 6 3 7, and dimension 8 e + n of a group of 32 values is column
@@ -570,7 +571,7 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
           tc_wait_st();
         }
         if (grow) m_ref = m_true;
-        const float mb = m_ref == -CUDART_INF_F ? 0.f : -m_ref * c2;
+        const float mb = m_ref == -CUDART_INF_F ? 0.f : fmaf(-m_ref, c2, kProbShift);
         float rs[2] = {0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < 4; c += 2) {          // probabilities take the places of the logits they come from
@@ -602,7 +603,7 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
       if (!ok) break;
       tc_fence_after();
       const int row = i * kChM + r;
-      const float rel = l > 0.f ? ex2((m_ref - m_true) * c2) : 1.f;       // results relative to the row's true maximum
+      const float rel = l > 0.f ? ex2((m_ref - m_true) * c2) * kProbUnshift : 1.f;       // results relative to the row's true maximum
       const float f = s.whole ? (l > 0.f ? 1.f / l : 1.f) : rel;
       float* part = s.whole ? nullptr : split_part(a, gridDim.x, kChRows, blockIdx.x, s.part);
       Segment sg;

@@ -12,8 +12,9 @@
 // dimensions are multiplied by their scale in 32 bits.  Queries are scaled to a largest magnitude in [2^14, 2^15) per row (a power of two;
 // bf16 has 8 bits, fp16 11, so only elements 2^-20 below the row's largest lose any) and the pairs whose codes arrive 16 times too large are
 // divided by 16.  All of it is exact but for the 32-bit sums.
-// Outputs: values times scales are exact in fp16; probabilities are rounded to fp16 (2^-11, an eighth of the output's own rounding).
-// The block's reference maximum of a row moves only when a row's maximum outgrows it by 2^8, so probabilities stay far below 65504.
+// Outputs: values times scales are exact in fp16; probabilities are rounded to fp16, by 2^-11 (an eighth of the output's own rounding) down to
+// 2^-21 of the row's reference, by 2^-32 of the reference below (kProbShift): those of a million keys that all vanish are 2^-12 of the sum.
+// The block's reference maximum of a row moves only when a row's maximum outgrows it by 2^8, so what becomes fp16 stays below 2^15.
 // Bound by instruction issue: about 480 instructions per 16 keys of a group, issued every second clock.  Without unpacking and products the same
 // loop takes 145 us for 64 requests of up to 32000 tokens (93 % of the copy bandwidth), with them 236.
 #include <algorithm>
@@ -321,7 +322,7 @@ __global__ void __launch_bounds__(kMmThreads, MmaSmem<GK, GV>::kBlocksPerSm) cac
       uint32_t p[2][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float b = st.m[h] == -CUDART_INF_F ? 0.f : -st.m[h] * st.c2[h];
+        const float b = st.m[h] == -CUDART_INF_F ? 0.f : fmaf(-st.m[h], st.c2[h], kProbShift);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const float e0 = ex2(fmaf(x[t][2 * h], st.c2[h], b)), e1 = ex2(fmaf(x[t][2 * h + 1], st.c2[h], b));
@@ -407,7 +408,7 @@ __global__ void __launch_bounds__(kMmThreads, MmaSmem<GK, GV>::kBlocksPerSm) cac
         const float2 h0 = ml[0][r], h1 = ml[1][r], h2 = ml[2][r], h3 = ml[3][r];
         sum[h] = (h0.y + h1.y) + (h2.y + h3.y);
         top[h] = max_of_row(fmaxf(fmaxf(h0.x, h1.x), fmaxf(h2.x, h3.x)), sum[h]);
-        const float rel = top[h] == -CUDART_INF_F ? 0.f : ex2((st.m[h] - top[h]) * st.c2[h]);       // to the row's true maximum
+        const float rel = top[h] == -CUDART_INF_F ? 0.f : ex2((st.m[h] - top[h]) * st.c2[h]) * kProbUnshift;       // to the row's true maximum
         const float M = top[h] == -CUDART_INF_F ? top[h] : top[h] * st.cl[h];
         f[h] = whole ? (sum[h] > 0.f ? 1.f / sum[h] : sum[h]) : rel;
         if (whole) {

@@ -253,3 +253,42 @@ def test_block_tables_of_lengths_beyond_reason(S, page, seed):
 @pytest.mark.parametrize("seed", [27, 1171, 1241, 1892, 1958])
 def test_block_tables_of_sums_that_would_wrap(seed):
     _check_bounded(*_wrapping_lengths(seed), 64, 64)
+
+
+# ------------------------------------------------------------------------------------------------ one key far above many
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,new", [(BF, 1), (BF, 16), (F32, 1)])
+@pytest.mark.parametrize("heads", HEADS)
+def test_one_key_far_above_a_long_tail(dtype, new, heads):
+    """A first key whose logit is 12 to 21 above those of 50 000 others, in segments that a block has whole: what the others add up to is
+    still there, each off by no more than 2^-32 of the first.  (Its own value is 0, so nothing else shows.)"""
+    from types import SimpleNamespace
+
+    from nsa.paged import PagedCache4
+    H, G, dk, dv = heads
+    hp, T = H // G, 50000
+    S = (592 if new == 1 else 148) // G                     # as many segments of one length as there are thread blocks
+    pages = -(-T // 64)
+    c = PagedCache4.empty(pages, G, dk, dv)
+    k, v = torch.zeros(T, G, dk, device="cuda"), torch.ones(T, G, dv, device="cuda")
+    k[0], v[0] = 1, 0
+    slots = torch.arange(T, device="cuda")
+    c.append(k, v, slots)
+    k, v = c.read(slots)
+    up = torch.linspace(12, 21, hp, device="cuda").repeat(G) / dk ** 0.5          # logit = up * dk * dk^-1/2
+    q = up[None, :, None].expand(new, H, dk).to(dtype).contiguous()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    table = torch.arange(pages, device="cuda", dtype=torch.int32).repeat(S, 1)
+    o, L, M = c.attend(q.repeat(S, 1, 1), table, i32([T] * S), i32([new * r for r in range(S + 1)]))
+    for x in (o, L, M):
+        assert torch.equal(x.view(S, new, *x.shape[1:]), x[:new].expand(S, *x[:new].shape))
+    s = SimpleNamespace(lengths=[T], starts=[0, new], dk=dk, k=[k], v=[v])
+    want = by_request(s, q)
+    ref.check((o[:new], L[:new], M[:new]), want, dtype, T, dk)
+    ro, rL, rM, A, B, V = want
+    # the probabilities' own roundings are 2^-11; logits and 32-bit sums as in ref.check
+    rel = 2 * (dk * 2.0 ** -24 * B + 2.0 ** -23 * rM) + T * 2.0 ** -24 + 2.0 ** -22 + (2.0 ** -11 if dtype == BF else 0)
+    tol = rel[..., None] * A + (2.0 ** -8 if dtype == BF else 2.0 ** -23) * ro + (2.0 ** -32 * V if dtype == BF else 0)
+    err = (o[:new].double() - ro).abs()
+    assert bool((err <= tol).all()), f"off by up to {(err / tol).max().item():.3g} of the bound"
