@@ -51,7 +51,7 @@ constexpr int kChPieces = 4, kChRoleWarps = 13;
 struct ChunkBarriers {
   uint64_t piece_full[kChPieces], piece_empty[kChPieces];
   ChunkPiece piece[kChPieces];
-  uint64_t q_full[2], k_full, k_empty, v_full[2], v_empty[2], s_full[2], p_half[2], p_full[2], pv_done[2], o_free[2];
+  uint64_t q_full[2], k_full, k_empty, v_full[2], v_empty[2], s_full[2], p_half[2], p_full[2], pv_done[2], o_free[2], drained;
   long long scratch[kChThreads / 32 + 3];
   uint32_t tmem_base;
   int abort;
@@ -144,6 +144,7 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
     }
     mbar_init(&bar->k_full, 128);
     mbar_init(&bar->k_empty, 1);
+    mbar_init(&bar->drained, 1);
     bar->abort = 0;
     fence_barrier_init();
     fence_proxy_async();
@@ -304,6 +305,11 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
         }
         ++ic0;
         if (two) ++ic1;
+      }
+      if (__any_sync(0xffffffffu, *abort)) {        // products in flight end before the block gives its memory back, or another limit ends that
+        volatile int overdue = 0;
+        commit(leader, &bar->drained);
+        mbar_wait_warp(&bar->drained, 0, &overdue);
       }
     }
   } else if (warp >= 8) {
@@ -669,6 +675,7 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
 
   // ------------------------------------------------------------ teardown (every thread gets here)
   pdl_launch();
+  asm volatile("cp.async.wait_all;" ::: "memory");        // (queries that a wait which ran out left on their way)
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && bar->abort) report_timeout(timeouts);

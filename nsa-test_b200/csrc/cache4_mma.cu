@@ -364,9 +364,10 @@ __global__ void __launch_bounds__(kMmThreads, MmaSmem<GK, GV>::kBlocksPerSm) cac
       }
     }
     __syncthreads();
-    if (*abort) {               // let copies in flight land before the block gives its shared memory back
+    if (*abort) {               // copies in flight land before the block gives its shared memory back, or another limit ends that (`abort` would at once)
+      volatile int overdue = 0;
       for (; threadIdx.x == 0 && done < unit; ++done) {
-        mbar_wait(&full[i], phase, abort);
+        mbar_wait(&full[i], phase, &overdue);
         if (++i == kMmStages) {
           i = 0;
           phase ^= 1;
