@@ -21,6 +21,9 @@ constexpr int kHeldRequests = 4096, kHeldBytes = kHeldRequests * 8;
 // Probabilities that become fp16 are 2^7 times what they are against a row's reference: the reference lags by 2^8 at most, so they stay below
 // 65504, and fp16 ends at 2^-32 of the reference instead of 2^-25.  (Sums have the factor too; results take it out.)
 constexpr float kProbShift = 7.f, kProbUnshift = 0.0078125f;
+// An exponent is one multiply-add, x c2 - (m c2): rounding the product in brackets moves all of a row's by the same 2^-25 of it, which cancels.
+// From here on it would be places of its own (and fp16 overflow): x - m comes first then, and is exact where it matters.
+constexpr float kFarLogit = 0x1p20f;       // log2 units
 
 struct Segment {
   int tok0;        // first token of the request among the step's (selected form: the token)

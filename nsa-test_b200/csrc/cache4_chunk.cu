@@ -559,25 +559,46 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
         const bool first = m_ref == -CUDART_INF_F;
         const bool grow = first ? m_true > m_ref : m_true > m_ref + thr;
         const bool need_o = grow && !first;
-        if (__any_sync(0xffffffffu, need_o)) {
-          ok = mbar_wait_warp(&bar->pv_done[i], (sc + t - 1) & 1, abort);   // O_i must hold PV(t - 1) before it is scaled
-          if (!ok) break;
-          tc_fence_after();
-          const float f = need_o ? ex2((m_ref - m_true) * c2) : 1.f;
-          l *= f;
+        const float m_new = grow ? m_true : m_ref, mc = m_new * c2;
+        const bool far = fabsf(mc) > kFarLogit && m_new > -CUDART_INF_F;
+        float mb = m_new == -CUDART_INF_F ? 0.f : kProbShift - mc;
+        if (__any_sync(0xffffffffu, need_o || far)) {
+          if (__any_sync(0xffffffffu, need_o)) {
+            ok = mbar_wait_warp(&bar->pv_done[i], (sc + t - 1) & 1, abort);   // O_i must hold PV(t - 1) before it is scaled
+            if (!ok) break;
+            tc_fence_after();
+            const float f = need_o ? ex2((m_ref - m_true) * c2) : 1.f;
+            l *= f;
 #pragma unroll 2
-          for (int c = 0; c < DV / 8; ++c) {
-            uint32_t ov[8];
-            tmem_ld8(tO + c * 8, ov);
-            tc_wait_ld();
+            for (int c = 0; c < DV / 8; ++c) {
+              uint32_t ov[8];
+              tmem_ld8(tO + c * 8, ov);
+              tc_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * f);
-            tmem_st8(tO + c * 8, ov);
+              for (int e = 0; e < 8; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * f);
+              tmem_st8(tO + c * 8, ov);
+            }
+            tc_wait_st();
           }
-          tc_wait_st();
+          if (__any_sync(0xffffffffu, far)) {
+            const float m = far ? m_new : 0.f;
+            if (far) mb = kProbShift;
+#pragma unroll 1
+            for (int c = 0; c < kChN; c += 32) {     // (by way of tensor memory: code that hardly ever runs stays short)
+              uint32_t x[32];
+              tmem_ld32(tS + c, x);
+              tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) - m);
+              tmem_st32(tS + c, x);
+            }
+            tc_wait_st();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, sv[c]);
+            tc_wait_ld();
+          }
         }
-        if (grow) m_ref = m_true;
-        const float mb = m_ref == -CUDART_INF_F ? 0.f : fmaf(-m_ref, c2, kProbShift);
+        m_ref = m_new;
         float rs[2] = {0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < 4; c += 2) {          // probabilities take the places of the logits they come from

@@ -245,6 +245,7 @@ __global__ void __launch_bounds__(kMmThreads, MmaSmem<GK, GV>::kBlocksPerSm) cac
     load_rows<GK>(a, s, smem + SM::oQ, sc, st);
     __syncthreads();
     int done = 0;
+    bool far = false;           // some row of this warp has logits beyond kFarLogit
     for (; done < units; ++done) {
       ok = mbar_wait_warp(&full[i], phase, abort);
       // ---- this warp's 16 keys: sums x [tile of 8 keys][row n: keys 2 j, 2 j + 1; row n + 8: the same]
@@ -318,11 +319,18 @@ __global__ void __launch_bounds__(kMmThreads, MmaSmem<GK, GV>::kBlocksPerSm) cac
             }
           }
         }
+        far = __any_sync(0xffffffffu, fmaxf(st.m[0] * st.c2[0], st.m[1] * st.c2[1]) > kFarLogit ||
+                                          (st.m[0] > -CUDART_INF_F && st.m[0] * st.c2[0] < -kFarLogit) ||
+                                          (st.m[1] > -CUDART_INF_F && st.m[1] * st.c2[1] < -kFarLogit));
+      }
+      if (far) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e >> 2][e & 3] -= st.m[e >> 1 & 1] == -CUDART_INF_F ? 0.f : st.m[e >> 1 & 1];
       }
       uint32_t p[2][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float b = st.m[h] == -CUDART_INF_F ? 0.f : fmaf(-st.m[h], st.c2[h], kProbShift);
+        const float b = st.m[h] == -CUDART_INF_F ? 0.f : far ? kProbShift : fmaf(-st.m[h], st.c2[h], kProbShift);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const float e0 = ex2(fmaf(x[t][2 * h], st.c2[h], b)), e1 = ex2(fmaf(x[t][2 * h + 1], st.c2[h], b));

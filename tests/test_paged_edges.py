@@ -292,3 +292,25 @@ def test_one_key_far_above_a_long_tail(dtype, new, heads):
     tol = rel[..., None] * A + (2.0 ** -8 if dtype == BF else 2.0 ** -23) * ro + (2.0 ** -32 * V if dtype == BF else 0)
     err = (o[:new].double() - ro).abs()
     assert bool((err <= tol).all()), f"off by up to {(err / tol).max().item():.3g} of the bound"
+
+
+# ------------------------------------------------------------------------------------------------ large logits
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 3, 40])
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("size", [1e6, 1e8, 1e10, 1e20])
+def test_large_queries(new, heads, size):
+    """Logits of 1e6 to 1e21: hardly more than the largest key counts."""
+    s = Served([300], [new], *heads, BF, seed=41)
+    H, G, dk, _ = heads
+    s.q.mul_(size)
+    o, L, M = s.check()
+    x = torch.einsum("nghd,tgd->nght", s.q.double().unflatten(1, (G, H // G)), s.k[0].double()).reshape(new, H, 300) * dk ** -0.5
+    near = torch.einsum("nghd,tgd->nght", s.q.double().abs().unflatten(1, (G, H // G)), s.k[0].double().abs()).reshape(new, H, 300).amax(-1) * dk ** -0.5
+    x = x.masked_fill(torch.arange(300, device="cuda") > 300 - new + torch.arange(new, device="cuda")[:, None, None], -math.inf)
+    top, at = x.topk(2, -1)
+    sure = top[..., 0] - top[..., 1] > 2 * dk * 2.0 ** -24 * near + 1000          # further apart than a logit is off
+    assert sure.float().mean() > 0.9
+    first = s.v[0][at[..., 0], torch.arange(H, device="cuda") // (H // G)]           # [new, H, dv]
+    assert torch.equal(o[sure], first[sure].bfloat16()) and not L[sure].any() and M.isfinite().all()
