@@ -511,7 +511,9 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
       const ChunkPiece& s = bar->piece[cur % kChPieces];
       const int n = s.n, p0 = s.p0;
       const int row0 = s.row0 + i * kChM, my_pos = pos;
-      const float c2 = cl * kLog2e, thr = kChGrow / c2, row_cl = cl;
+      // held within 2^-100 and 2^80, so that S (at most 2^39) times it is finite and -inf times it is -inf: beyond, values of S that differ at
+      // all are worlds apart or all are one
+      const float c2 = fminf(fmaxf(cl * kLog2e, 0x1p-100f), 0x1p80f), thr = kChGrow / c2, row_cl = cl;
       const int minpos = s.pos0 + row0 / a.hpg, maxpos = s.pos0 + (s.row0 + min(s.nrows, (i + 1) * kChM) - 1) / a.hpg;
       float m_true = -CUDART_INF_F, m_ref = -CUDART_INF_F, l = 0.f;
       int id0, id1;

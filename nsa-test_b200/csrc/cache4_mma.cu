@@ -63,7 +63,7 @@ __device__ __forceinline__ uint32_t code_bits(uint32_t x, uint32_t mask) {      
 // what a warp keeps of a segment; the lane holds rows n and n + 8
 struct MmaState {
   float o[4][4];                               // 32 dimensions of the outputs
-  float m[2], lim[2], top[2], l[2], c2[2], cl[2];      // lim: what a maximum has to exceed for m to move; c2, cl: a unit of the sums in log2 and natural logits
+  float m[2], lim[2], top[2], l[2], c2[2], cl[2];      // lim: what a maximum has to exceed for m to move; c2: a unit of the sums in log2 logits; cl: 2^24 of them in logits
   int pos[2];
 };
 
@@ -94,8 +94,10 @@ __device__ __forceinline__ void load_rows(const Cache4Args& a, const Segment& s,
     const int k = mx ? min(14 - ((int)(mx >> 7) - 127), 100) : 0;
     // the scale's sign goes into the row, so that a larger sum is always the larger logit; scale 0 is a row of zeros
     up[h] = mx >= 0x7f80 ? CUDART_NAN_F : __uint_as_float((uint32_t)(k + 127) << 23) * (a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f);
-    st.cl[h] = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * __uint_as_float((uint32_t)(127 - k) << 23) * 16777216.f;
-    st.c2[h] = st.cl[h] * kLog2e;
+    st.cl[h] = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * __uint_as_float((uint32_t)(127 - k) << 23);
+    // Held within 2^100 either way, so that a sum (at most 2^15) times it is finite and -inf times it is -inf: beyond, sums that differ at all
+    // are worlds apart or all sums are one.
+    st.c2[h] = fminf(fmaxf(st.cl[h] * (16777216.f * kLog2e), 0x1p-100f), 0x1p100f);
     st.m[h] = st.lim[h] = st.top[h] = -CUDART_INF_F;
     st.l[h] = 0.f;
   }
@@ -418,7 +420,7 @@ __global__ void __launch_bounds__(kMmThreads, MmaSmem<GK, GV>::kBlocksPerSm) cac
         sum[h] = (h0.y + h1.y) + (h2.y + h3.y);
         top[h] = max_of_row(fmaxf(fmaxf(h0.x, h1.x), fmaxf(h2.x, h3.x)), sum[h]);
         const float rel = top[h] == -CUDART_INF_F ? 0.f : ex2((st.m[h] - top[h]) * st.c2[h]) * kProbUnshift;       // to the row's true maximum
-        const float M = top[h] == -CUDART_INF_F ? top[h] : top[h] * st.cl[h];
+        const float M = top[h] == -CUDART_INF_F ? top[h] : top[h] * 16777216.f * st.cl[h];
         f[h] = whole ? (sum[h] > 0.f ? 1.f / sum[h] : sum[h]) : rel;
         if (whole) {
           const int64_t row = out_row(a, s, r);

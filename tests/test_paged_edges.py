@@ -294,14 +294,14 @@ def test_one_key_far_above_a_long_tail(dtype, new, heads):
     assert bool((err <= tol).all()), f"off by up to {(err / tol).max().item():.3g} of the bound"
 
 
-# ------------------------------------------------------------------------------------------------ large logits
+# ------------------------------------------------------------------------------------------------ queries and scales at the ends of their range
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("new", [1, 3, 40])
 @pytest.mark.parametrize("heads", HEADS)
-@pytest.mark.parametrize("size", [1e6, 1e8, 1e10, 1e20])
+@pytest.mark.parametrize("size", [1e6, 1e8, 1e10, 1e20, 1e33, 1e36])
 def test_large_queries(new, heads, size):
-    """Logits of 1e6 to 1e21: hardly more than the largest key counts."""
+    """Logits of 1e6 to 1e37: hardly more than the largest key counts."""
     s = Served([300], [new], *heads, BF, seed=41)
     H, G, dk, _ = heads
     s.q.mul_(size)
@@ -314,3 +314,20 @@ def test_large_queries(new, heads, size):
     assert sure.float().mean() > 0.9
     first = s.v[0][at[..., 0], torch.arange(H, device="cuda") // (H // G)]           # [new, H, dv]
     assert torch.equal(o[sure], first[sure].bfloat16()) and not L[sure].any() and M.isfinite().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_scales_near_zero(dtype, new):
+    """Scales down to the smallest numbers there are: the mean of what a row sees."""
+    s = Served([300, 70], [new, 1], *HEADS[2], dtype, seed=42)
+    for size in (1.0, 1e-30):
+        s.q.mul_(size)
+        for scale in (1e-12, 1e-25, 1e-38, 1e-44, -1e-30):
+            scale = torch.tensor(scale).item()              # (as 32 bits have it)
+            o, L, M = s.cache.attend(s.q, s.table, s.len_dev, s.starts_dev, scale=scale)
+            ro, rL, rM, A, B, V = by_request(s, s.q, scale=scale)
+            # 32 bits keep no relative precision below 2^-126: largest logits are off by as much besides what ref.check allows
+            assert bool(((M - rM).abs() <= 64 * 2.0 ** -24 * B + 2.0 ** -23 * rM.abs() + 2.0 ** -126).all())
+            ref.check((o, L, rM), (ro, rL, rM, A, B, V), dtype, 300, 64)
