@@ -62,7 +62,7 @@ struct Walk {
   static constexpr int kChunk = kHeldRequests;
   const Cache4Args& a;
   Segment s;
-  int tile, tiles, len, fresh;              // of the current request
+  int tile, tiles, len, fresh;              // of the current request (selected form: fresh is the first request's first token)
   long long total;
 
   __device__ Walk(const Cache4Args& args) : a(args) {}
@@ -158,7 +158,8 @@ struct Walk {
   template <int T>
   __device__ __forceinline__ void start(long long* scratch, long long* held) {
     if (SEL && a.n_sel) {
-      const int n = min(max(a.starts[a.S], 0), a.N);
+      fresh = min(max(a.starts[0], 0), a.N);
+      const int n = max(min(a.starts[a.S], a.N) - fresh, 0);
       tiles = (a.hpg + ROWS - 1) / ROWS;
       s.lo = 0;
       s.hi = a.n_sel;
@@ -188,7 +189,7 @@ struct Walk {
       const long long seg = quotient(u, length()), of_tiles = quotient(seg, tiles), of_groups = quotient(of_tiles, a.G);
       tile = (int)(seg - of_tiles * tiles);
       s.g = (int)(of_tiles - of_groups * a.G);
-      s.tok0 = (int)of_groups;
+      s.tok0 = fresh + (int)of_groups;
       int lo = 0, up = a.S;                     // last request that starts at or before the token: 32 probes at a time
       while (up - lo > 1) {
         const int step = (up - lo + 31) / 32, at = lo + lane * step;

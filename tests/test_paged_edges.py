@@ -331,3 +331,25 @@ def test_scales_near_zero(dtype, new):
             # 32 bits keep no relative precision below 2^-126: largest logits are off by as much besides what ref.check allows
             assert bool(((M - rM).abs() <= 64 * 2.0 ** -24 * B + 2.0 ** -23 * rM.abs() + 2.0 ** -126).all())
             ref.check((o, L, rM), (ro, rL, rM, A, B, V), dtype, 300, 64)
+
+
+# ------------------------------------------------------------------------------------------------ some of a step's requests
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,heads", [(BF, HEADS[0]), (BF, HEADS[2]), (F32, HEADS[2]), (BF, ODD_HEADS[0])])
+@pytest.mark.parametrize("form", ["all", "window", "selected"])
+@pytest.mark.parametrize("first,last", [(1, 5), (2, 4), (0, 3), (3, 3), (4, 5)])
+def test_some_requests_of_a_step(dtype, heads, form, first, last):
+    """Slices of the tables, lengths and starts of a step: only the rows of those requests are written."""
+    s = Served([200, 90, 64, 333, 70], [3, 1, 40, 2, 60], *heads, dtype, seed=50)
+    N, G = s.starts[-1], heads[1]
+    gen = torch.Generator().manual_seed(51)
+    kw = dict(window=33) if form == "window" else {}
+    if form == "selected":
+        kw = dict(indices=torch.randint(-1, 6, (N, G, 4), generator=gen, dtype=torch.int32).cuda())
+    want = ref.attend(s.q, s.k, s.v, s.lengths, s.starts, s.dk ** -0.5, **kw)
+    out = torch.full((N, heads[0], heads[3]), 5.0, device="cuda", dtype=dtype)
+    o, L, M = s.cache.attend(s.q, s.table[first:last], s.len_dev[first:last], s.starts_dev[first:last + 1], out=out, **kw)
+    a, b = s.starts[first], s.starts[last]
+    ref.check([x[a:b] for x in (o, L, M)], [x[a:b] for x in want], dtype, 333, s.dk) if a < b else None
+    assert (out[:a] == 5).all() and (out[b:] == 5).all()
