@@ -455,7 +455,8 @@ NSA_API int nsa_incremental_fwd(const nsa_decode_desc* desc, void* workspace, si
  * of the requests, and are written into the table.  slots and positions [N] list the new tokens one request after the other (-1 behind
  * the last, N is at least their number), starts [S + 1] where each request's begin, lengths [S] the tokens it then has, pages [1] how
  * many pages the step takes.  Where that is more than F, or a table row is too short, tokens without a page have slot -1 (and
- * table entries -1): the caller compares pages with F.  Negative lengths count as 0.  At most 16384 requests a call.
+ * table entries -1): the caller compares pages with F.  Negative lengths count as 0.  At most 16384 requests and 2^30 tokens a call, pages of
+ * 1 to 65536 tokens.
  *
  * nsa_cache4_append: k [N,G,dk] and v [N,G,dv] (strides6: token, group, dimension of each) into their slots; slots outside the cache are
  * passed over.  Slots of one call are distinct (a slot given twice holds bytes of both tokens).  nsa_cache4_read: the values that the

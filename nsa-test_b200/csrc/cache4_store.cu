@@ -404,6 +404,7 @@ extern "C" NSA_API int nsa_block_tables(const int32_t* cached, const int32_t* fr
                                         int64_t* slots, int32_t* positions, int32_t* starts, int32_t* lengths, int32_t* pages, int S, int P,
                                         int F, int N, int page, void* stream) {
   NSA_REQUIRE(S >= 0 && P >= 0 && F >= 0 && N >= 0 && table_ld >= P, "block_tables: bad sizes %d/%d/%d/%d", S, P, F, N);
+  NSA_REQUIRE(N <= 1 << 30, "block_tables: %d tokens, at most %d in one call", N, 1 << 30);
   NSA_REQUIRE(S <= kTblMaxRequests, "block_tables: %d requests, at most %d in one call", S, kTblMaxRequests);
   NSA_REQUIRE(page > 0 && page <= 65536, "block_tables: page size %d outside 1..65536", page);
   NSA_REQUIRE(starts && pages && (S == 0 || (cached && fresh && lengths)) && (S == 0 || P == 0 || table) && (F == 0 || free_pages) &&

@@ -25,6 +25,7 @@ __all__ = ["PAGE_TOKENS", "MAX_SELECTED", "StepTables", "block_tables", "PagedCa
 PAGE_TOKENS = 64
 MAX_SELECTED = 32
 _FLOATS = (torch.bfloat16, torch.float32)
+_MOST_TOKENS, _MOST_PAGE_TOKENS = 1 << 30, 1 << 16
 
 
 class StepTables(NamedTuple):
@@ -68,8 +69,8 @@ def block_tables(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, f
     _int32("free_pages", free_pages, (None,))
     if S > 1 and table.stride(0) < table.shape[1]:
         raise ValueError("table rows overlap")
-    if tokens < 0 or page_tokens < 1:
-        raise ValueError(f"tokens {tokens} and page_tokens {page_tokens} must not be negative or zero")
+    if not 0 <= tokens <= _MOST_TOKENS or not 1 <= page_tokens <= _MOST_PAGE_TOKENS:
+        raise ValueError(f"tokens {tokens} and page_tokens {page_tokens} must be 0 to {_MOST_TOKENS} and 1 to {_MOST_PAGE_TOKENS}")
     return StepTables(*ops.block_tables(cached, new, table, free_pages, int(tokens), int(page_tokens)))
 
 
@@ -153,7 +154,7 @@ class PagedCache4:
         if q.stride(2) != 1 or (q.dtype == torch.bfloat16 and (q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8)):
             q = q.clone(memory_format=torch.contiguous_format)      # the tensor-core kernels load rows 16 bytes at a time
         return ops.cache4_attn(q, self.storage, table, lengths, starts, indices, dk, dv, 0 if window is None else min(int(window), 1 << 30),
-                               1.0 / math.sqrt(dk) if scale is None else float(scale), 0 if max_new is None else int(max_new), out)
+                               1.0 / math.sqrt(dk) if scale is None else float(scale), 0 if max_new is None else min(int(max_new), 1 << 30), out)
 
     def _check_slots(self, slots: torch.Tensor, n: int) -> None:
         if slots.dtype != torch.int64 or slots.dim() != 1 or slots.shape[0] != n or (n > 1 and slots.stride(0) != 1):

@@ -353,3 +353,25 @@ def test_some_requests_of_a_step(dtype, heads, form, first, last):
     a, b = s.starts[first], s.starts[last]
     ref.check([x[a:b] for x in (o, L, M)], [x[a:b] for x in want], dtype, 333, s.dk) if a < b else None
     assert (out[:a] == 5).all() and (out[b:] == 5).all()
+
+
+# ------------------------------------------------------------------------------------------------ refusals (no GPU)
+
+def test_counts_beyond_32_bits():
+    """Counts that 32 bits would cut short are refused, not cut."""
+    from nsa import _lib as L
+    from nsa.paged import PagedCache4, block_tables
+    one, table = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 3, dtype=torch.int32)
+    for tokens, page in ((2 ** 32 + 2, 64), (2 ** 30 + 1, 64), (2, 2 ** 32 + 64), (2, 65537)):
+        with pytest.raises(ValueError, match="tokens"):
+            block_tables(one, one, table, one, tokens, page)
+    assert L.lib.nsa_block_tables(16, 16, 16, 4, 16, 16, 16, 16, 16, 16, 1, 4, 1, 2 ** 30 + 1, 64, None) == -1
+    c = PagedCache4.empty(2, 2, 64, 64, device="cpu")
+    with pytest.raises(RuntimeError):               # (a bound of any size is one: what is missing is the GPU)
+        c.attend(torch.zeros(3, 4, 64), table, one, torch.zeros(3, dtype=torch.int32), max_new=2 ** 40)
+
+
+@pytest.mark.gpu
+def test_a_bound_beyond_32_bits():
+    s = Served([90, 40], [30, 1], *HEADS[0], BF, seed=52)
+    s.check(max_new=2 ** 40)
