@@ -458,7 +458,8 @@ extern "C" NSA_API int nsa_cache4_attn_fwd(const nsa_cache4_desc* desc, void* wo
   Cache4Args a;
   if (int rc = cache4_args(desc, a)) return rc;
   if (a.N == 0 || a.S == 0) return NSA_OK;
-  NSA_REQUIRE(a.q && a.starts && a.lengths && a.out && a.L && a.M && (a.P == 0 || (a.table && a.table_ld >= a.P)) && (a.n_pages == 0 || a.cache) &&
+  NSA_REQUIRE(a.table_ld >= a.P, "cache4_attn: table rows %lld apart overlap, they have %d pages", (long long)a.table_ld, a.P);
+  NSA_REQUIRE(a.q && a.starts && a.lengths && a.out && a.L && a.M && (a.P == 0 || a.table) && (a.n_pages == 0 || a.cache) &&
                   (a.n_sel == 0 || a.indices), "cache4_attn: null pointer");
   NSA_REQUIRE((uintptr_t)a.cache % 16 == 0, "cache4_attn: the cache must be 16-byte aligned");
   const size_t need = nsa_cache4_attn_workspace_bytes(desc);

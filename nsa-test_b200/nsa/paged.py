@@ -139,6 +139,8 @@ class PagedCache4:
             raise ValueError(f"table must be int32 [S, P], got {tuple(table.shape)}")
         S = table.shape[0]
         _int32("table", table, (S, None))
+        if S > 1 and table.stride(0) < table.shape[1]:
+            raise ValueError("table rows overlap")
         _int32("lengths", lengths, (S,))
         _int32("starts", starts, (S + 1,))
         if window is not None and (window < 1 or indices is not None):

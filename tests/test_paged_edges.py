@@ -375,3 +375,19 @@ def test_counts_beyond_32_bits():
 def test_a_bound_beyond_32_bits():
     s = Served([90, 40], [30, 1], *HEADS[0], BF, seed=52)
     s.check(max_new=2 ** 40)
+
+
+def test_table_rows_that_overlap():
+    from nsa import _lib as L
+    from nsa.paged import PagedCache4
+    i32 = dict(dtype=torch.int32)
+    c = PagedCache4.empty(2, 2, 64, 64, device="cpu")
+    q, lengths, starts = torch.zeros(2, 4, 64), torch.ones(2, **i32), torch.arange(3, **i32)
+    for table in (torch.zeros(1, 3, **i32).expand(2, 3), torch.zeros(5, **i32).as_strided((2, 3), (2, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            c.attend(q, table, lengths, starts)
+    with pytest.raises(RuntimeError):               # a row of its own needs no distance
+        c.attend(q[:1], torch.zeros(1, 3, **i32).expand(1, 3), lengths[:1], starts[:2])
+    d = dict(N=1, S=2, P=3, H=4, G=2, dk=64, dv=64, n_pages=1, n_sel=0, window=0, max_new=0, dtype=1, scale=1.0, s0=256, s1=64, ld=2, q=16, cache=16,
+             table=16, lengths=16, starts=16, indices=0, out=16, L=16, M=16)
+    assert L.lib.nsa_cache4_attn_fwd(L.CACHE4_DESC.pack(*d.values()), 16, 1 << 40, None) == -1 and b"overlap" in L.lib.nsa_last_error()
