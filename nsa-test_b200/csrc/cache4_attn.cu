@@ -374,8 +374,10 @@ constexpr int kFmaRows = 8;
 constexpr int kC4Smem = 227 * 1024 - 4096;
 
 // Rows (new tokens times heads of a group) from which a request goes to the tensor-memory kernel: it does 256 rows for the price of one,
-// the mma.sync kernel 16 at a time.  Head dims 192/128, 16 requests of 8000 tokens: 48 rows 69 us against 63, 64 rows 70 against 79, 96 rows
-// 69 against 110; with short caches (a window of 512, 64 rows) 28 against 25, and its fixed cost makes one request of 300 tokens 22 against 14.
+// the mma.sync kernel 16 at a time.  us, it against the mma.sync kernel:
+//   16 requests of up to 8000 tokens, 48 / 64 / 80 / 96 rows   192/128: 70:63 71:80 71:98 72:114   128/128: 41:36 41:43 41:52 41:58   64/64: 33:30 33:35 33:41 32:46
+//   32 requests, a window of 512, 64 / 80 / 96 rows            192/128: 41:39 42:46 42:51          128/128: 30:26 30:32 30:34         64/64: 25:24 26:29 26:31
+// Where there are few keys in all its fixed cost loses: one request of 300 tokens, 64 to 128 rows, 22:12, 21:11 and 18:10.
 constexpr int kChunkRows = 80;
 
 // records in flight; at first the requests' units are held there

@@ -16,7 +16,7 @@
 //
 // Bound by the round trip of a tile: softmax about 2100 clocks (1024 of them the exponentials of 128 keys alone, shared with the other tile's
 // warps), its own two products 1280 at head dims 192/128, handing over on either side of both 400 to 900; about 4400 clocks for two tiles of
-// 128 keys, where the tensor pipe needs 2560.  2048 new tokens behind 30000 earlier ones, 16 query heads a group, 4 groups: 2.2 ms (1150 TFLOP/s)
+// 128 keys, where the tensor pipe needs 2560.  2000 new tokens behind 30000 earlier ones, 16 query heads a group, 4 groups: 2.1 ms (1200 TFLOP/s)
 // on a chip that is not warm; a long loop of it is slowed by the power limit (2.3 to 2.5 ms).
 #include <algorithm>
 

@@ -15,8 +15,10 @@
 // Outputs: values times scales are exact in fp16; probabilities are rounded to fp16, by 2^-11 (an eighth of the output's own rounding) down to
 // 2^-21 of the row's reference, by 2^-32 of the reference below (kProbShift): those of a million keys that all vanish are 2^-12 of the sum.
 // The block's reference maximum of a row moves only when a row's maximum outgrows it by 2^8, so what becomes fp16 stays below 2^15.
-// Bound by instruction issue: about 480 instructions per 16 keys of a group, issued every second clock.  Without unpacking and products the same
-// loop takes 145 us for 64 requests of up to 32000 tokens (93 % of the copy bandwidth), with them 236.
+// What bounds it: no unit is full.  470 instructions per 16 keys of a group (about 280 of them unpack and multiply, the rest is a page's own: masks,
+// growth, exchange, fetch) take 45 % of the issue slots and the tensor pipe is active a third of the time; with 16 warps an SM what
+// shows is fixed latencies, the two barriers of a page, the math pipes and the fetching of code.  64 requests of up to 32000 tokens: 240 us; without
+// unpacking and products the same loop takes 145 (93 % of the copy bandwidth).
 #include <algorithm>
 
 #include "attn_args.cuh"

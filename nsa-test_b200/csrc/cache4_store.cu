@@ -27,9 +27,9 @@ __device__ __forceinline__ int add(int x, int y) { return min(x + y, (1 << 30) -
 // Every block forms the prefix sums of all requests' new tokens and new pages (8 bytes a request out of L2, far less than what a
 // second launch or a wait between blocks costs), then deals with its own 512 tokens.  A token whose position opens a page takes
 // that page off the free list and writes it into the table; old entries are only read, so no two threads touch one place.
-// Bound by the launch and dependent reads (the sums, a search per token, the table): 2.7 us for 256 requests of one token, 4.4 us for 45 000
-// tokens of 1000 requests (10 us with 2048 tokens a block).  512 threads take half the steps over many requests (5.4 us with 256), up
-// to 256 requests they only cost their start (3.1 us).
+// Bound by the launch and dependent reads (the sums, a search per token, the table): 3.1 us for 256 requests of one token, 4.8 us for 45 000
+// tokens of 1000 requests (7.3 us with 2048 tokens a block).  512 threads take half the steps over many requests (with 256 the second case
+// takes 5.9 us), up to 256 requests they only cost their start (the first case 3.4 us).
 __global__ void __launch_bounds__(kTblMaxThreads) block_tables_kernel(const TablesArgs a) {
   extern __shared__ int32_t sm_tbl[];
   int32_t* first_tok = sm_tbl;                  // [S + 1]
