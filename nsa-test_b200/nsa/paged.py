@@ -58,7 +58,8 @@ def block_tables(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, f
     ``table [S,P]`` holds the pages of each request's cached tokens and receives those that the new ones open, taken from the front of
     ``free_pages`` in the order of the requests.  ``tokens`` is the number of new tokens or, where that is not known on the host (a
     captured graph), a bound of it.  Lengths are data on the GPU, so a free list or a table row that is too short raises nothing: the tokens
-    without a page get slot -1, which the cache passes over, and ``pages`` says how many the step needed.
+    without a page get slot -1, which the cache passes over, and ``pages`` says how many the step needed.  At most 16384 requests and 2^30
+    tokens a call, pages of 1 to 65536 tokens.
     """
     if table.dim() != 2:
         raise ValueError(f"table must be int32 [S, P], got {tuple(table.shape)}")
