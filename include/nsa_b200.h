@@ -467,7 +467,8 @@ NSA_API int nsa_incremental_fwd(const nsa_decode_desc* desc, void* workspace, si
  * n_sel > 0 those in the 64-key blocks indices[token][group][0..n_sel) (int32, contiguous; negative ones and repetitions do not count),
  * n_sel <= 32.  Pages that the table does not give (entries outside 0..n_pages-1, positions behind its P pages) are not seen.  out [N,H,dv]
  * contiguous in the type of q; L, M [N,H] as above; rows that see nothing are 0, L = M = -inf; rows whose query has a NaN or an infinity are
- * NaN in all three if they see anything.  Rows behind the last request's are left as they were.  max_new: no request has more new tokens than this (0: not known); it only chooses between kernels. */
+ * NaN in all three if they see anything.  Rows behind the last request's are left as they were.  max_new: no request has more new tokens than this (0: not known); it only chooses between kernels.
+ * scale is finite. */
 NSA_API int nsa_block_tables(const int32_t* cached, const int32_t* fresh, int32_t* table, int64_t table_ld, const int32_t* free_pages,
                              int64_t* slots, int32_t* positions, int32_t* starts, int32_t* lengths, int32_t* pages, int S, int P, int F,
                              int N, int page_tokens, void* stream);

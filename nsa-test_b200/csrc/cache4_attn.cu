@@ -1,5 +1,6 @@
 // Attention of a step's queries over the 4-bit paged cache: see cache4_attn.cuh for how the work is cut up.
 #include <algorithm>
+#include <cmath>
 
 #include "attn_args.cuh"
 #include "cache4_attn.cuh"
@@ -427,6 +428,7 @@ static int cache4_args(const nsa_cache4_desc* d, Cache4Args& a) {
   NSA_REQUIRE(d->n_sel >= 0 && d->n_sel <= kSelMax, "cache4_attn: %d selected blocks, at most %d", d->n_sel, kSelMax);
   NSA_REQUIRE(d->window >= 0 && (d->window == 0 || d->n_sel == 0), "cache4_attn: a window and selected blocks do not go together");
   NSA_REQUIRE(d->max_new >= 0, "cache4_attn: negative max_new");
+  NSA_REQUIRE(std::isfinite(d->scale), "cache4_attn: scale %g is not finite", (double)d->scale);
   NSA_REQUIRE(d->P <= 1 << 23, "cache4_attn: %d pages a request, at most %d", d->P, 1 << 23);
   NSA_REQUIRE((int64_t)d->N * d->H <= 0x7fffffffll / 4, "cache4_attn: %d tokens of %d heads in one call", d->N, d->H);
   a.q = d->q; a.cache = (const uint8_t*)d->cache; a.table = d->table; a.lengths = d->lengths; a.starts = d->starts;

@@ -154,6 +154,8 @@ class PagedCache4:
             raise ValueError(f"attend: out must be contiguous {q.dtype} [{q.shape[0]}, {q.shape[1]}, {dv}]")
         if max_new is not None and max_new < 0:
             raise ValueError("attend: negative max_new")
+        if scale is not None and not math.isfinite(scale):
+            raise ValueError(f"attend: scale {scale} is not finite")
         if q.stride(2) != 1 or (q.dtype == torch.bfloat16 and (q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8)):
             q = q.clone(memory_format=torch.contiguous_format)      # the tensor-core kernels load rows 16 bytes at a time
         return ops.cache4_attn(q, self.storage, table, lengths, starts, indices, dk, dv, 0 if window is None else min(int(window), 1 << 30),

@@ -391,3 +391,16 @@ def test_table_rows_that_overlap():
     d = dict(N=1, S=2, P=3, H=4, G=2, dk=64, dv=64, n_pages=1, n_sel=0, window=0, max_new=0, dtype=1, scale=1.0, s0=256, s1=64, ld=2, q=16, cache=16,
              table=16, lengths=16, starts=16, indices=0, out=16, L=16, M=16)
     assert L.lib.nsa_cache4_attn_fwd(L.CACHE4_DESC.pack(*d.values()), 16, 1 << 40, None) == -1 and b"overlap" in L.lib.nsa_last_error()
+
+
+def test_scales_that_are_not_finite():
+    from nsa import _lib as L
+    from nsa.paged import PagedCache4
+    i32 = dict(dtype=torch.int32)
+    c = PagedCache4.empty(2, 2, 64, 64, device="cpu")
+    d = dict(N=1, S=1, P=3, H=4, G=2, dk=64, dv=64, n_pages=1, n_sel=0, window=0, max_new=0, dtype=1, scale=1.0, s0=256, s1=64, ld=3, q=16, cache=16,
+             table=16, lengths=16, starts=16, indices=0, out=16, L=16, M=16)
+    for scale in (math.nan, math.inf, -math.inf):
+        with pytest.raises(ValueError, match="scale"):
+            c.attend(torch.zeros(1, 4, 64), torch.zeros(1, 3, **i32), torch.ones(1, **i32), torch.arange(2, **i32), scale=scale)
+        assert L.lib.nsa_cache4_attn_fwd(L.CACHE4_DESC.pack(*{**d, "scale": scale}.values()), 16, 1 << 40, None) == -1 and b"scale" in L.lib.nsa_last_error()
