@@ -404,3 +404,28 @@ def test_scales_that_are_not_finite():
         with pytest.raises(ValueError, match="scale"):
             c.attend(torch.zeros(1, 4, 64), torch.zeros(1, 3, **i32), torch.ones(1, **i32), torch.arange(2, **i32), scale=scale)
         assert L.lib.nsa_cache4_attn_fwd(L.CACHE4_DESC.pack(*{**d, "scale": scale}.values()), 16, 1 << 40, None) == -1 and b"scale" in L.lib.nsa_last_error()
+
+
+# ------------------------------------------------------------------------------------------------ offsets beyond 32 bits
+
+@pytest.mark.gpu
+def test_pages_behind_4_gigabytes():
+    """The last pages of a cache of 6 GB: the same bits as in a small one, written, read and attended to."""
+    from nsa.paged import PagedCache4
+    H, G, dk, dv = HEADS[0]
+    pages = 130000
+    big = PagedCache4(torch.empty(pages, G, 64 * 180, device="cuda", dtype=torch.uint8), dk, dv)
+    assert big.storage.numel() > 5 << 30
+    for dtype, new in ((BF, 1), (BF, 20), (F32, 2)):
+        s = Served([700, 90], [new, 1], H, G, dk, dv, dtype, seed=53)
+        n = s.cache.storage.shape[0]
+        table = torch.where((s.table >= 0) & (s.table < n), s.table + (pages - n), s.table)
+        for r, length in enumerate(s.lengths):
+            pos = torch.arange(length, device="cuda")
+            slots = table[r, pos // 64].long() * 64 + pos % 64
+            big.append(s.k[r], s.v[r], slots)              # (what the small cache holds is held exactly again)
+            assert all(torch.equal(x, y) for x, y in zip(big.read(slots), (s.k[r], s.v[r])))
+        idx = torch.randint(-1, 12, (s.starts[-1], G, 5), dtype=torch.int32).cuda()
+        for kw in ({}, dict(window=70), dict(indices=idx)):
+            want = s.cache.attend(s.q, s.table, s.len_dev, s.starts_dev, **kw)
+            assert all(torch.equal(x, y) for x, y in zip(want, big.attend(s.q, table, s.len_dev, s.starts_dev, **kw)))
