@@ -515,7 +515,8 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
       // all are worlds apart or all are one
       const float c2 = fminf(fmaxf(cl * kLog2e, 0x1p-100f), 0x1p80f), thr = kChGrow / c2, row_cl = cl;
       const int minpos = s.pos0 + row0 / a.hpg, maxpos = s.pos0 + (s.row0 + min(s.nrows, (i + 1) * kChM) - 1) / a.hpg;
-      float m_true = -CUDART_INF_F, m_ref = -CUDART_INF_F, l = 0.f;
+      float m_true = -CUDART_INF_F, m_ref = -CUDART_INF_F, l = 0.f, mb = 0.f;      // mb: kProbShift less the reference
+      bool far = false;                  // the row has logits beyond kFarLogit
       int id0, id1;
       pages_of(s, p0, id0, id1);
       for (int t = 0; t < n && ok; ++t) {
@@ -561,15 +562,18 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
         const bool first = m_ref == -CUDART_INF_F;
         const bool grow = first ? m_true > m_ref : m_true > m_ref + thr;
         const bool need_o = grow && !first;
-        const float m_new = grow ? m_true : m_ref, mc = m_new * c2;
-        const bool far = fabsf(mc) > kFarLogit && m_new > -CUDART_INF_F;
-        float mb = m_new == -CUDART_INF_F ? 0.f : kProbShift - mc;
+        const float m_old = m_ref;
+        if (grow) {
+          m_ref = m_true;
+          far = fabsf(m_ref * c2) > kFarLogit;
+          mb = far ? kProbShift : kProbShift - m_ref * c2;
+        }
         if (__any_sync(0xffffffffu, need_o || far)) {
           if (__any_sync(0xffffffffu, need_o)) {
             ok = mbar_wait_warp(&bar->pv_done[i], (sc + t - 1) & 1, abort);   // O_i must hold PV(t - 1) before it is scaled
             if (!ok) break;
             tc_fence_after();
-            const float f = need_o ? ex2((m_ref - m_true) * c2) : 1.f;
+            const float f = need_o ? ex2((m_old - m_ref) * c2) : 1.f;
             l *= f;
 #pragma unroll 2
             for (int c = 0; c < DV / 8; ++c) {
@@ -583,8 +587,7 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
             tc_wait_st();
           }
           if (__any_sync(0xffffffffu, far)) {
-            const float m = far ? m_new : 0.f;
-            if (far) mb = kProbShift;
+            const float m = far ? m_ref : 0.f;
 #pragma unroll 1
             for (int c = 0; c < kChN; c += 32) {     // (by way of tensor memory: code that hardly ever runs stays short)
               uint32_t x[32];
@@ -600,7 +603,6 @@ __global__ void __launch_bounds__(kChThreads, 1) cache4_chunk_kernel(const Cache
             tc_wait_ld();
           }
         }
-        m_ref = m_new;
         float rs[2] = {0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < 4; c += 2) {          // probabilities take the places of the logits they come from

@@ -17,7 +17,7 @@
 // The block's reference maximum of a row moves only when a row's maximum outgrows it by 2^8, so what becomes fp16 stays below 2^15.
 // What bounds it: no unit is full.  470 instructions per 16 keys of a group (about 280 of them unpack and multiply, the rest is a page's own: masks,
 // growth, exchange, fetch) take 45 % of the issue slots and the tensor pipe is active a third of the time; with 16 warps an SM what
-// shows is fixed latencies, the two barriers of a page, the math pipes and the fetching of code.  64 requests of up to 32000 tokens: 240 us; without
+// shows is fixed latencies, the two barriers of a page, the math pipes and the fetching of code.  64 requests of up to 32000 tokens: 238 us; without
 // unpacking and products the same loop takes 145 (93 % of the copy bandwidth).
 #include <algorithm>
 
@@ -250,6 +250,7 @@ __global__ void __launch_bounds__(kMmThreads, MmaSmem<GK, GV>::kBlocksPerSm) cac
     __syncthreads();
     int done = 0;
     bool far = false;           // some row of this warp has logits beyond kFarLogit
+    float bias[2] = {0.f, 0.f}; // of the exponents: kProbShift less the reference
     for (; done < units; ++done) {
       ok = mbar_wait_warp(&full[i], phase, abort);
       // ---- this warp's 16 keys: sums x [tile of 8 keys][row n: keys 2 j, 2 j + 1; row n + 8: the same]
@@ -323,9 +324,12 @@ __global__ void __launch_bounds__(kMmThreads, MmaSmem<GK, GV>::kBlocksPerSm) cac
             }
           }
         }
-        far = __any_sync(0xffffffffu, fmaxf(st.m[0] * st.c2[0], st.m[1] * st.c2[1]) > kFarLogit ||
-                                          (st.m[0] > -CUDART_INF_F && st.m[0] * st.c2[0] < -kFarLogit) ||
-                                          (st.m[1] > -CUDART_INF_F && st.m[1] * st.c2[1] < -kFarLogit));
+        float mc[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) mc[h] = st.m[h] == -CUDART_INF_F ? 0.f : st.m[h] * st.c2[h];
+        far = __any_sync(0xffffffffu, fmaxf(fabsf(mc[0]), fabsf(mc[1])) > kFarLogit);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) bias[h] = far ? kProbShift : kProbShift - mc[h];
       }
       if (far) {
 #pragma unroll
@@ -334,10 +338,9 @@ __global__ void __launch_bounds__(kMmThreads, MmaSmem<GK, GV>::kBlocksPerSm) cac
       uint32_t p[2][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float b = st.m[h] == -CUDART_INF_F ? 0.f : far ? kProbShift : fmaf(-st.m[h], st.c2[h], kProbShift);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const float e0 = ex2(fmaf(x[t][2 * h], st.c2[h], b)), e1 = ex2(fmaf(x[t][2 * h + 1], st.c2[h], b));
+          const float e0 = ex2(fmaf(x[t][2 * h], st.c2[h], bias[h])), e1 = ex2(fmaf(x[t][2 * h + 1], st.c2[h], bias[h]));
           st.l[h] += e0 + e1;
           p[t][h] = as_u32(__floats2half2_rn(e0, e1));
         }
